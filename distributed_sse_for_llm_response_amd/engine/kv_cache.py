@@ -13,6 +13,8 @@ from __future__ import annotations
 
 import torch
 
+from .. import ops
+
 PAGE = 32
 
 
@@ -21,6 +23,10 @@ class KVCache:
         self.num_layers, self.num_blocks, self.nkv = num_layers, num_blocks, nkv
         self.k = torch.zeros(num_layers, num_blocks, nkv, PAGE, 128, device=device, dtype=dtype)
         self.v = torch.zeros(num_layers, num_blocks, nkv, 128, PAGE, device=device, dtype=dtype)
+
+    def pools(self) -> list:
+        """The page tensors as ``ops.page_fork`` copies them, [layers, pages, ..]."""
+        return [self.k, self.v]
 
     @staticmethod
     def bytes_per_block(num_layers: int, nkv: int) -> int:
@@ -78,6 +84,10 @@ class LatentKVCache:
     def __getitem__(self, li: int) -> torch.Tensor:
         return self.layers[li]
 
+    def pools(self) -> list:
+        """The page tensors as ``ops.page_fork`` copies them, [1, pages, ..]."""
+        return [t[None] for group in (self.layers, self.vt) for t in group.values()]
+
     @staticmethod
     def bytes_per_block(widths: dict, elem_bytes: int = 2) -> int:
         return max(1, sum(widths.values()) * PAGE * elem_bytes)
@@ -101,6 +111,11 @@ class RecurrentStateCache:
             for t in group.values():
                 t.index_copy_(0, dst_idx, t.index_select(0, src_idx))
 
+    def reorder(self, parents: torch.Tensor, width: int) -> None:
+        """Every slot takes the state of slot parents[s] (int32, one per slot, within its group of `width` slots), in place: the
+        beams of a search change places."""
+        ops.state_reorder([t for group in (self.state, self.tail) for t in group.values()], parents, width)
+
 
 class PagedKVCache:
     """Paged keys and values of softmax-attention layers with any head widths: per attention run one key tensor
@@ -117,6 +132,10 @@ class PagedKVCache:
         # 16-byte load per lane; decode steps read the row-major pages
         self.vt = {r: torch.zeros(num_blocks, shapes[r][0], shapes[r][2], PAGE, device=device, dtype=dtype)
                    for r in transposed}
+
+    def pools(self) -> list:
+        """The page tensors as ``ops.page_fork`` copies them, [1, pages, ..]."""
+        return [t[None] for group in (self.k, self.v, self.vt) for t in group.values()]
 
     @staticmethod
     def bytes_per_block(shapes: dict, elem_bytes: int = 2) -> int:
@@ -145,6 +164,9 @@ class MixedKVCache:
         self.num_blocks = num_blocks
         self.latent = LatentKVCache(latent_widths, num_blocks, device, dtype, transposed=latent_transposed)
         self.paged = PagedKVCache(kv_shapes, num_blocks, device, dtype, transposed=kv_transposed)
+
+    def pools(self) -> list:
+        return self.latent.pools() + self.paged.pools()
 
 
 class ConvTailCache(RecurrentStateCache):
@@ -176,3 +198,7 @@ class MemoryStateCache(RecurrentStateCache):
         super().move(src_idx, dst_idx)
         for t in self.norm.values():
             t.index_copy_(0, dst_idx, t.index_select(0, src_idx))
+
+    def reorder(self, parents: torch.Tensor, width: int) -> None:
+        super().reorder(parents, width)
+        ops.state_reorder(list(self.norm.values()), parents, width)

@@ -347,3 +347,4 @@ from .layers import (conv_state, embed_rows, gate_math, gate_pair, gated_act, ga
                      sink_flash_ok, sink_flash_lds, sink_tile_rows, sink_decode_ok, moe_route_rows, stream_step, stream_mix, act_rows, moe_route, embed_pair_rows, add_norm_rows,
                      token_gate_rows, token_side_rows, token_side_fits, qkv_rows, conv_qkv_rows,
                      matrix_memory, memory_chunk_ok, memory_work_floats, moe_table_lists)
+from .beams import BEAM_KEEP, BEAM_WIDTH, FORK_SLOTS, beam_attention, beam_select, beam_shared, page_fork, state_reorder  # noqa: E402,F401

@@ -1,0 +1,499 @@
+"""A beam search's kernels (selection over beams and vocabulary, attention over shared pages, forks of block tables, states that change
+slots) against their references in 64 bits, which the CPU tests hold against definitions of their own."""
+import math
+
+import pytest
+import torch
+
+from distributed_sse_for_llm_response_amd import ops
+from distributed_sse_for_llm_response_amd.engine import kv_cache
+from distributed_sse_for_llm_response_amd.ops import beams_reference as bref
+from distributed_sse_for_llm_response_amd.ops.reference import gather_kv
+
+pytestmark = pytest.mark.gpu
+INF = math.inf
+
+
+# ------------------------------------------------------------------------------------------------------------ selection
+# A row's log-sum: each exponential has an argument y in (-42, 0] rounded twice (|y| 2^-23) and one step of its own (2^-23), what is
+# below 2^-42 of the largest counts for nothing; a value goes through at most 80 additions (2^-24 each).  The score rounds once.
+LOG_SUM = 43 * 2.0 ** -23 + 80 * 2.0 ** -24
+
+
+def _logits(gen, rows, V, dtype):
+    """Multiples of 1/8, exact in both types: many equal logits in a row, while scores of different rows are told apart by their
+    log-sums and base scores."""
+    return (torch.randn(rows, V, generator=gen) * 16).round().clamp(-120, 120).div(8).to(dtype)
+
+
+def _apart(logits, scores):
+    """Whether no two rows' scores are as near as two log-sums may be off (modulo the logits' steps of 1/8)."""
+    z = torch.logsumexp(logits.double(), 1)
+    off = (scores.double().flatten() - z).view(scores.shape)
+    for row in off:
+        f = sorted(float(v) % 0.125 for v in row if math.isfinite(v))
+        if any(b - a < 2.1 * LOG_SUM for a, b in zip(f, f[1:])) or (len(f) > 1 and f[0] + 0.125 - f[-1] < 2.1 * LOG_SUM):
+            return False
+    return True
+
+
+def _scores(gen, logits, groups, width, most):
+    """Base scores that keep the rows apart."""
+    while True:
+        scores = -torch.rand(groups, width, generator=gen) * most
+        if _apart(logits, scores):
+            return scores
+
+
+def _select(dev, logits, scores, K, eos=-1):
+    G, W = scores.shape
+    outs = []
+    for f, d in ((bref.beam_select, "cpu"), (ops.beam_select, dev)):
+        o = (torch.full((G, K), 7.0, device=d), torch.full((G, K), 7, device=d, dtype=torch.int32),
+             torch.full((G, K), 7, device=d, dtype=torch.int32))
+        end = torch.full((G, W), 7.0, device=d) if eos >= 0 else None
+        f(logits.cpu() if d == "cpu" else logits, scores.to(d), *o, eos, end)
+        outs.append([t.cpu() for t in o] + ([end.cpu()] if eos >= 0 else []))
+    return outs
+
+
+def _same_choice(want, got):
+    assert torch.equal(want[1], got[1]) and torch.equal(want[2], got[2])
+    for a, b in zip([want[0]] + want[3:], [got[0]] + got[3:]):
+        live = a > -INF
+        assert torch.equal(live, b > -INF)
+        a, b = a[live].double(), b[live].double()
+        assert bool(((a - b).abs() <= LOG_SUM + 2 * 2.0 ** -24 * a.abs()).all()), float((a - b).abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("groups,width,V,K", [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 63, 64), (1, 4, 1000, 4), (3, 5, 2048, 10),
+                                              (1, 8, 32768, 16), (2, 32, 4099, 64), (1, 2, 50001, 3), (5, 4, 777, 8), (1, 3, 9000, 33)])
+def test_select(gpu, dtype, groups, width, V, K):
+    gen = torch.Generator().manual_seed(1000 * groups + V + K)
+    logits = _logits(gen, groups * width, V, dtype)
+    scores = _scores(gen, logits, groups, width, 9)
+    for eos in {-1, V // 2, V - 1}:
+        _same_choice(*_select(gpu, logits.to(gpu), scores, K, eos))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("start", [1, 2, 3, 5])
+def test_select_strided_rows(gpu, dtype, start):
+    """Rows of a wider buffer at addresses of every alignment."""
+    gen = torch.Generator().manual_seed(start)
+    wide = _logits(gen, 8, 5003, dtype).to(gpu)
+    logits = wide[:, start: start + 4700]
+    scores = _scores(gen, logits.cpu(), 2, 4, 5)
+    _same_choice(*_select(gpu, logits, scores, 8, 17))
+
+
+def test_select_equal_logits(gpu):
+    """Every token equal: the first tokens of the best row, in order; of two equal rows the first one's."""
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.full((4, 9001), 0.5, device=gpu, dtype=dtype)
+        want, got = _select(gpu, logits, torch.tensor([[-2.0, -1.0, -1.0, -3.0]]), 64)
+        assert got[1].tolist() == [[1] * 64] and got[2].tolist() == [list(range(64))]
+        _same_choice(want, got)
+        want, got = _select(gpu, logits[:, :40], torch.tensor([[-2.0, -1.0, -1.0, -3.0]]), 64)
+        assert got[1].tolist() == [[1] * 40 + [2] * 24]
+        _same_choice(want, got)
+
+
+def test_select_what_is_not_finite(gpu):
+    gen = torch.Generator().manual_seed(3)
+    logits = _logits(gen, 12, 3000, torch.float32)
+    scores = _scores(gen, logits, 2, 6, 1)
+    logits[1, 7] = math.nan          # a row with NaN, with +inf, of -inf alone, of two values only
+    logits[2, 2999] = INF
+    logits[3] = -INF
+    logits[4, 5:] = -INF
+    logits[4, :3] = -INF
+    logits[6:, ::2] = -INF
+    logits[8] = torch.finfo(torch.float32).min   # masked by the type's lowest value throughout, and in part
+    logits[9, 10:] = torch.finfo(torch.float32).min
+    scores[0, 5], scores[1, 1], scores[1, 5] = -INF, math.nan, INF
+    for eos in (-1, 3, 7):
+        _same_choice(*_select(gpu, logits.to(gpu), scores, 16, eos))
+    scores.fill_(-INF)
+    _, got = _select(gpu, logits.to(gpu), scores, 16, 3)
+    assert bool((got[0] == -INF).all()) and bool((got[1] == -1).all()) and bool((got[2] == -1).all()) and bool((got[3] == -INF).all())
+
+
+@pytest.mark.parametrize("V", [4096, 40000])
+def test_select_best_in_one_lane(gpu, V):
+    """The best tokens 256 or 1024 apart, where a workgroup's lanes meet the same few: the bound of the chunk's best is low then, and
+    a long list is gathered."""
+    for step in (4, 256, 1024, 2048):
+        logits = torch.zeros(1, V)
+        logits[0, ::step] = 20 + torch.arange(0, V, step).flip(0) / 8192
+        _same_choice(*_select(gpu, logits.to(gpu), torch.tensor([[-1.0]]), 64))
+
+
+def test_select_more_candidates_than_gathered(gpu):
+    """One row of 32 far ahead: the merge meets all of the group's best in few lists."""
+    V = 40960
+    logits = torch.zeros(32, V)
+    logits[5] = torch.linspace(0, 4, V)
+    logits[6] = torch.linspace(4, 0, V)
+    scores = torch.full((1, 32), -500.0) - torch.arange(32) * 3
+    scores[0, 5], scores[0, 6] = -1.0, -1.01
+    _same_choice(*_select(gpu, logits.to(gpu), scores, 64))
+
+
+def test_select_first_step_and_graph(gpu):
+    """One beam in use, then a captured selection replayed over new logits."""
+    gen = torch.Generator().manual_seed(9)
+    logits = _logits(gen, 8, 2500, torch.float32).to(gpu)
+    scores = torch.tensor([[-0.5, -INF, -INF, -INF], [-INF, -INF, -1.5, -INF]])
+    _same_choice(*_select(gpu, logits, scores, 4, 2))
+    o = (torch.empty(2, 4, device=gpu), torch.empty(2, 4, device=gpu, dtype=torch.int32), torch.empty(2, 4, device=gpu, dtype=torch.int32))
+    s = scores.to(gpu)
+    ops.beam_select(logits, s, *o, 2)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.beam_select(logits, s, *o, 2)
+    for seed in range(4):
+        gen = torch.Generator().manual_seed(20 + seed)
+        new = _logits(gen, 8, 2500, torch.float32)
+        sc = _scores(gen, new, 2, 4, 4)
+        logits.copy_(new)
+        s.copy_(sc)
+        g.replay()
+        torch.cuda.synchronize()
+        want, got = _select(gpu, logits, sc, 4, 2)
+        _same_choice(want[:3], [t.cpu() for t in o])
+        _same_choice(want, got)
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+def _cache(gen, pages, hkv, dev):
+    k = torch.randn(pages, hkv, 32, 128, generator=gen).to(torch.bfloat16)
+    v = torch.randn(pages, hkv, 128, 32, generator=gen).to(torch.bfloat16)
+    return k.to(dev), v.to(dev)
+
+
+def _tables(gen, lens, common, width, extra=1):
+    """Block tables of groups whose beams have common[g] leading pages the same and the others their own, in random order."""
+    S = len(lens)
+    need = [max(common[s // width], -(-n // 32)) for s, n in enumerate(lens)]
+    total = sum(common) + sum(n - common[s // width] for s, n in enumerate(need)) + 3
+    perm, at = torch.randperm(total, generator=gen).tolist(), 0
+    bt = torch.zeros(S, max(need) + extra, dtype=torch.int32)
+    for g in range(S // width):
+        for j in range(common[g]):
+            bt[g * width: (g + 1) * width, j] = perm[at]
+            at += 1
+    for s in range(S):
+        for j in range(common[s // width], need[s]):
+            bt[s, j] = perm[at]
+            at += 1
+    return bt, total
+
+
+def _attend(dev, gen, lens, common, width, hq, hkv, poison=False):
+    bt, pages = _tables(gen, lens, common, width)
+    k, v = _cache(gen, pages, hkv, "cpu")
+    if poison:  # what stands in a page past the sequence's end is not finite
+        for s, n in enumerate(lens):
+            if n % 32:
+                t = torch.arange(n % 32, 32)
+                k[int(bt[s, n // 32])][:, t] = math.nan
+                v[int(bt[s, n // 32])][:, :, ((t & 15) >> 2) * 8 + (t >> 4) * 4 + (t & 3)] = INF
+    q = torch.randn(len(lens), hq, 128, generator=gen).to(torch.bfloat16)
+    ctx = torch.tensor(lens, dtype=torch.int32)
+    shared = torch.zeros(len(lens) // width, dtype=torch.int32)
+    bref.beam_shared(bt, ctx, width, shared)
+    dsh = torch.full_like(shared, -5).to(dev)
+    ops.beam_shared(bt.to(dev), ctx.to(dev), width, dsh)
+    assert torch.equal(dsh.cpu(), shared)
+    out = torch.full(q.shape, 3.0, dtype=torch.bfloat16, device=dev)
+    args = (q.to(dev), k.to(dev), v.to(dev), bt.to(dev), ctx.to(dev))
+    ops.beam_attention(*args, dsh, out, width)
+    # weights and result round to bf16 (half a step, 2^-8, each); a score is 128 products of some 0.1 summed in 32 bits
+    for s, n in enumerate(lens):
+        got = out[s].cpu().double()
+        if n == 0:
+            assert bool((got == 3.0).all())
+            continue
+        K, V = (x.double().repeat_interleave(hq // hkv, 1) for x in gather_kv(k, v, bt[s], n))
+        p = torch.softmax((q[s].double()[None] * K).sum(-1) / math.sqrt(128), 0)[..., None]
+        want, size = (p * V).sum(0), (p * V.abs()).sum(0)
+        assert bool(((got - want).abs() <= (2.0 ** -8 + 1e-4) * size + 2.0 ** -8 * want.abs()).all()), (s, float((got - want).abs().max()))
+    return args, dsh, out
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (8, 4), (32, 8), (8, 1), (16, 1), (12, 4), (5, 1)])
+@pytest.mark.parametrize("width", [1, 3, 4, 8])
+def test_attention_heads(gpu, hq, hkv, width):
+    gen = torch.Generator().manual_seed(hq * 100 + width)
+    lens = [97 + 13 * s for s in range(2 * width)]
+    _attend(gpu, gen, lens, [2, 3], width, hq, hkv)
+
+
+@pytest.mark.parametrize("width,lens,common", [
+    (2, [1, 1], [0]), (2, [1, 0], [0]), (2, [0, 0, 5, 31], [0, 0]), (4, [32, 32, 32, 32], [1]), (4, [33, 32, 64, 65], [1]),
+    (3, [64, 65, 66, 0, 0, 0, 40, 0, 90], [2, 0, 1]), (2, [4000, 4001], [120]), (2, [4000, 4001], [0]), (16, [700] * 16, [20]),
+    (32, [100 + i for i in range(32)], [3]), (1, [2500, 31, 1], [0, 0, 0])])
+def test_attention_lengths(gpu, width, lens, common):
+    gen = torch.Generator().manual_seed(sum(lens) + width)
+    _attend(gpu, gen, lens, common, width, 8, 2)
+
+
+def test_attention_past_the_end_not_finite(gpu):
+    gen = torch.Generator().manual_seed(4)
+    _attend(gpu, gen, [70, 65, 64, 83, 0, 95, 31, 161], [2, 0], 4, 8, 2, poison=True)  # no end lies in a page that others read
+
+
+def test_attention_shared_is_a_choice(gpu):
+    """Any number of pages up to the common ones gives the same numbers, more than are whole counts as those."""
+    gen = torch.Generator().manual_seed(5)
+    args, dsh, out = _attend(gpu, gen, [300, 290, 320, 310], [8], 4, 8, 2)
+    for n in (0, 1, 5, 9, 10 ** 6, -3):
+        o = torch.zeros_like(out)
+        ops.beam_attention(*args, torch.tensor([min(n, 8) if n < 10 ** 6 else 8], dtype=torch.int32, device=gpu), o, 4)
+        assert float((o.float() - out.float()).abs().max()) < 0.03
+    same = torch.zeros(1, 40, dtype=torch.int32).expand(4, 40).contiguous().to(gpu)
+    a, b = torch.zeros_like(out), torch.zeros_like(out)  # equal tables: pages that are not whole in every slot are not shared
+    ops.beam_attention(args[0], args[1], args[2], same, args[4], torch.tensor([40], dtype=torch.int32, device=gpu), a, 4)
+    ops.beam_attention(args[0], args[1], args[2], same, args[4], torch.tensor([9], dtype=torch.int32, device=gpu), b, 4)
+    assert torch.equal(a, b)
+
+
+def test_attention_as_paged_attention(gpu):
+    """Groups of one: the decode attention that the engine runs."""
+    gen = torch.Generator().manual_seed(6)
+    lens = [513, 40, 700, 1]
+    args, _, out = _attend(gpu, gen, lens, [0] * 4, 1, 8, 2)
+    i32 = dict(dtype=torch.int32, device=gpu)
+    o = torch.empty_like(out)
+    e = torch.empty(1, device=gpu)
+    ops.paged_attention(0, *args[:4], torch.arange(4, **i32), torch.ones(4, **i32), args[4], torch.arange(4, **i32), torch.zeros(4, **i32),
+                        o, e, e, 1024, 1)
+    assert float((o.float() - out.float()).abs().max()) < 0.03
+
+
+def test_attention_graph_and_stream(gpu):
+    gen = torch.Generator().manual_seed(7)
+    args, dsh, out = _attend(gpu, gen, [200, 210, 190, 220], [4], 2 * 2, 8, 2)
+    side = torch.cuda.Stream()
+    o = torch.zeros_like(out)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.beam_attention(*args, dsh, o, 4)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(o, out)
+    graphs = []
+    for _ in range(2):  # two graphs of the same call have work areas of their own
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.beam_attention(*args, dsh, o, 4)
+        graphs.append(g)
+    for n in (150, 220, 35):
+        args[4].copy_(torch.tensor([n, n + 1, n, n - 3], dtype=torch.int32))
+        ops.beam_shared(args[3], args[4], 4, dsh)
+        want = torch.zeros_like(out)
+        ops.beam_attention(*args, dsh, want, 4)
+        for g in graphs:
+            o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, want)
+
+
+# ---------------------------------------------------------------------------------------------------------------- forks
+def _fork_state(gen, lens, common, width, spare, M=None):
+    bt, used = _tables(gen, lens, common, width, extra=2)
+    if M is not None:
+        bt = bt[:, :M].contiguous()
+    held = torch.tensor([-(-n // 32) for n in lens], dtype=torch.int32)
+    refs = torch.zeros(used - 3 + spare, dtype=torch.int32)
+    # the tables' pages are a part of [0, used): number them anew, so that `spare` pages are free
+    pages = sorted({int(bt[s, j]) for s in range(len(lens)) for j in range(int(held[s]))})
+    places = torch.randperm(refs.numel(), generator=gen)[: len(pages)].tolist()
+    new = dict(zip(pages, places))
+    for s in range(len(lens)):
+        for j in range(bt.shape[1]):
+            bt[s, j] = new[int(bt[s, j])] if j < int(held[s]) else 0
+            if j < int(held[s]):
+                refs[int(bt[s, j])] += 1
+    return [bt, held, torch.tensor(lens, dtype=torch.int32)], refs
+
+
+def _fork(dev, state, refs, parents, pools):
+    S = state[0].shape[0]
+    sides = []
+    for f, d in ((bref.page_fork, "cpu"), (ops.page_fork, dev)):
+        t = [x.clone().to(d) for x in state] + [torch.tensor(parents, dtype=torch.int32, device=d), refs.clone().to(d),
+                                                torch.full((S, 2), 9, dtype=torch.int32, device=d),
+                                                torch.full((1,), 9, dtype=torch.int32, device=d)]
+        p = [x.clone().to(d) for x in pools]
+        f(*t, p)
+        sides.append([x.cpu() for x in t + p])
+    for a, b in zip(*sides):
+        assert torch.equal(a, b)
+    return sides[0]
+
+
+def _pools(gen, pages):
+    return [torch.randn(2, pages, 3, 32, 8, generator=gen).to(torch.bfloat16), torch.randn(1, pages, 32, 4, generator=gen),
+            torch.randint(0, 255, (3, pages, 16), generator=gen, dtype=torch.uint8)]
+
+
+@pytest.mark.parametrize("lens,common,width,parents", [
+    ([40, 40], [1], 2, [0, 0]), ([40, 40], [1], 2, [1, 0]), ([40, 40], [1], 2, [-1, 1]), ([40, 40], [1], 2, [-1, -1]),
+    ([64, 64, 64], [2], 3, [2, 2, 2]), ([64, 64, 64], [2], 3, [0, 1, 2]), ([96, 96, 96, 96], [1], 4, [3, 0, 0, -1]),
+    ([1, 0, 0, 0], [0], 4, [0, 0, 0, 0]), ([70, 0, 0, 0], [0], 4, [0, 0, 0, 0]), ([33, 65, 97, 129] * 4, [0, 0, 1, 1], 4, list(range(15, -1, -1))),
+    ([500 + s // 8 for s in range(80)], [15] * 10, 8, [8 * (s // 8) + (s * 5 + 3) % 8 // 2 for s in range(80)]),
+    ([31] * 6, [0], 6, [99, -7, 2, 2, 6, 5])])
+def test_fork(gpu, lens, common, width, parents):
+    gen = torch.Generator().manual_seed(len(lens) + sum(lens))
+    state, refs = _fork_state(gen, lens, common, width, 2 * len(lens) + 5)
+    pools = _pools(gen, refs.numel())
+    got = _fork(gpu, state, refs, parents, pools)
+    live = [s for s, q in enumerate(parents) if 0 <= q < len(lens)]
+    at = [int(got[0][s, int(got[2][s]) // 32]) for s in live]
+    assert len(set(at)) == len(at) and all(int(got[4][p]) == 1 for p in at) and int(got[6]) == 0
+    held = torch.zeros_like(got[4])
+    for s in range(len(lens)):
+        for j in range(int(got[1][s])):
+            held[int(got[0][s, j])] += 1
+    assert torch.equal(held, got[4])
+
+
+@pytest.mark.parametrize("spare", [0, 1, 2, 3])
+def test_fork_without_room(gpu, spare):
+    """Pages run out: who finds none keeps sharing, and a second call once pages are free serves them."""
+    gen = torch.Generator().manual_seed(spare)
+    state, refs = _fork_state(gen, [40, 41, 64, 64], [1], 4, spare)
+    pools = _pools(gen, refs.numel())
+    got = _fork(gpu, state, refs, [0, 0, 2, 0], pools)
+    freed = 2  # slots 1 and 3 give a page of their own up
+    assert int(got[6]) == max(0, 3 - spare - freed)
+    again = _fork(gpu, got[:3], got[4], [0, 1, 2, -1], got[7:])
+    assert int(again[6]) <= int(got[6])
+
+
+def test_fork_full_tables_and_other_holders(gpu):
+    gen = torch.Generator().manual_seed(11)
+    state, refs = _fork_state(gen, [128, 128, 100, 97], [2, 2], 2, 6, M=4)
+    _fork(gpu, state, refs, [1, 1, 2, 2], _pools(gen, refs.numel()))   # slots 0 and 1 have no further page
+    refs[int(state[0][2, 3])] += 1                                     # somebody else holds slot 2's last page too
+    got = _fork(gpu, state, refs, [0, 1, 2, 2], _pools(gen, refs.numel()))
+    assert int(got[5][2, 0]) == int(got[5][3, 0]) == int(state[0][2, 3])
+
+
+def test_fork_entries_that_are_no_pages(gpu):
+    """Ids outside the pool are carried along, count nowhere and are copied nowhere."""
+    gen = torch.Generator().manual_seed(12)
+    state, refs = _fork_state(gen, [70, 70], [2], 2, 6)
+    t = [x.clone().to(gpu) for x in state]
+    t[0][0, 2], t[0][1, 0] = 10 ** 6, -4
+    r = refs.to(gpu)
+    pools = [p.to(gpu) for p in _pools(gen, refs.numel())]
+    before = [p.clone() for p in pools]
+    copies, starved = torch.zeros(2, 2, dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+    ops.page_fork(*t, torch.tensor([0, 0], dtype=torch.int32, device=gpu), r, copies, starved, pools)
+    assert copies.tolist() == [[-1, -1], [-1, -1]] and all(torch.equal(a, b) for a, b in zip(pools, before))
+
+
+def test_fork_many_slots_and_pages(gpu):
+    gen = torch.Generator().manual_seed(13)
+    S, W = 2048, 8
+    lens = [35 + 3 * (s // W) % 60 for s in range(S)]
+    state, refs = _fork_state(gen, lens, [1] * (S // W), W, 20000)
+    parents = [W * (s // W) + int(x) for s, x in enumerate(torch.randint(0, W, (S,), generator=gen))]
+    parents[5 * W: 6 * W] = [-1] * W
+    _fork(gpu, state, refs, parents, [torch.randn(1, refs.numel(), 8, generator=gen)])
+
+
+def test_fork_many_pools_and_a_graph(gpu):
+    gen = torch.Generator().manual_seed(14)
+    state, refs = _fork_state(gen, [40, 45, 50, 55], [1], 4, 40)
+    pools = [torch.randn(1, refs.numel(), 4, generator=gen) for _ in range(130)]
+    _fork(gpu, state, refs, [2, 2, 0, 3], pools)
+    t = [x.clone().to(gpu) for x in state] + [torch.arange(4, dtype=torch.int32, device=gpu), refs.clone().to(gpu),
+                                              torch.zeros(4, 2, dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu)]
+    dp = [p.to(gpu) for p in pools[:3]]
+    ops.page_fork(*t, dp)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.page_fork(*t, dp)
+    now, r, p = [x.cpu() for x in t[:3]], t[4].cpu(), [x.cpu() for x in dp]
+    for parents in ([1, 1, 1, 3], [0, 0, 2, 2], [-1, 1, 1, 1], [1, 1, 2, 3]):
+        t[3].copy_(torch.tensor(parents, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        cpu = now + [torch.tensor(parents, dtype=torch.int32), r, torch.zeros(4, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)]
+        bref.page_fork(*cpu, p)
+        for a, b in zip(cpu + p, t + dp):
+            assert torch.equal(a, b.cpu())
+
+
+# --------------------------------------------------------------------------------------------------------------- states
+@pytest.mark.parametrize("width,groups", [(1, 3), (2, 5), (4, 1), (5, 3), (8, 2), (9, 2), (16, 1), (17, 2), (32, 1)])
+@pytest.mark.parametrize("kind", ["matrices", "odd", "halves"])
+def test_reorder(gpu, width, groups, kind):
+    gen = torch.Generator().manual_seed(width + groups)
+    S = width * groups
+    shapes = {"matrices": [(torch.float32, (4, 32, 16)), (torch.float32, (3, 96)), (torch.bfloat16, (64,))],
+              "odd": [(torch.float32, (3, 801)), (torch.float32, (5,)), (torch.float32, ())],
+              "halves": [(torch.bfloat16, (7,)), (torch.bfloat16, (3, 11)), (torch.float32, (9,))]}[kind]
+    for trial in range(4):
+        states = [torch.randn(S, *s, generator=gen).to(t) for t, s in shapes]
+        parents = width * (torch.arange(S) // width) + torch.randint(0, width, (S,), generator=gen)
+        if trial == 1:
+            parents = width * (torch.arange(S) // width) + (torch.arange(S) + 1) % width  # a cycle
+        if trial == 2:
+            parents[::3] = -1
+        if trial == 3:
+            parents = parents.flip(0)  # other groups' slots: left alone
+        parents = parents.to(torch.int32)
+        dev = [s.to(gpu) for s in states]
+        ops.state_reorder(dev, parents.to(gpu), width)
+        bref.state_reorder(states, parents, width)
+        for a, b in zip(states, dev):
+            assert torch.equal(a, b.cpu())
+
+
+def test_reorder_views_and_many(gpu):
+    """Slots of a wider buffer, more tensors than a launch takes, empty ones among them."""
+    gen = torch.Generator().manual_seed(2)
+    wide = torch.randn(6, 40, generator=gen)
+    states = [torch.randn(6, 1 + i % 7, generator=gen) for i in range(150)] + [torch.empty(6, 0), wide[:, 3:20]]
+    parents = torch.tensor([2, 0, 0, 3, 5, 4], dtype=torch.int32)
+    dw = wide.to(gpu)
+    dev = [s.to(gpu) for s in states[:-1]] + [dw[:, 3:20]]
+    ops.state_reorder(dev, parents.to(gpu), 3)
+    bref.state_reorder(states, parents, 3)
+    for a, b in zip(states, dev):
+        assert torch.equal(a, b.cpu())
+    assert torch.equal(dw.cpu(), wide)
+    ops.state_reorder([], parents.to(gpu), 3)
+
+
+def test_reorder_caches(gpu):
+    gen = torch.Generator().manual_seed(8)
+    parents = torch.tensor([1, 1, 0, 3, 7, 4, 4, 6], dtype=torch.int32)
+    for make in (lambda d: kv_cache.RecurrentStateCache({0: (160, 4), 3: (96, 2)}, 8, d),
+                 lambda d: kv_cache.MatrixStateCache({0: ((4, 32, 16), 0, 0), 1: ((2, 8, 8), 24, 4)}, 8, d),
+                 lambda d: kv_cache.MemoryStateCache({0: (2, 32, 64)}, {0: (64, 4)}, 8, d)):
+        a, b = make("cpu"), make(gpu)
+        for name in ("state", "tail", "norm"):
+            for key, t in getattr(a, name, {}).items():
+                t.copy_(torch.randn(t.shape, generator=gen))
+                getattr(b, name)[key].copy_(t)
+        a.reorder(parents, 4)
+        b.reorder(parents.to(gpu), 4)
+        for name in ("state", "tail", "norm"):
+            for key, t in getattr(a, name, {}).items():
+                assert torch.equal(t, getattr(b, name)[key].cpu())
+
+
+# ----------------------------------------------------------------------------------------------------------- all together
+def test_a_search(gpu):
+    from test_beams import check_search, search
+
+    check_search(search(gpu))
