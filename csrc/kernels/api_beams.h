@@ -24,7 +24,7 @@ struct BeamSelectParams {
   float2* cand;         // [rows, chunks, K] logit, token (bits); best first
   float* end_logit;     // [rows]
   int64_t ld;
-  int rows, width, V, K, eos, chunk, chunks, f32;
+  int rows, width, V, K, eos, pieces, chunks, f32;  // pieces of 16 bytes per thread; workgroups of a row
 };
 
 struct BeamAttnParams {
@@ -76,7 +76,7 @@ struct StateReorderParams {
 }  // namespace dsse
 
 extern "C" {
-int dsse_beam_chunk(int rows, int V, int f32, int whole);
+void dsse_beam_plan_rows(dsse::BeamSelectParams* p);  // pieces and chunks of the other fields
 hipError_t dsse_beam_select(const dsse::BeamSelectParams* p, hipStream_t st);
 void dsse_beam_plan(dsse::BeamAttnParams* p);  // tiles, col_blocks, ns, no of the other fields
 hipError_t dsse_beam_attention(const dsse::BeamAttnParams* p, hipStream_t st);

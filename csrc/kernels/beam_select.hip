@@ -17,9 +17,8 @@ namespace {
 
 constexpr int kSelThreads = 256;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kMergeCap = 2048;  // gathered candidates of a group that LDS holds
-
-DEV bool before(float a, int i, float b, int j) { return a > b || (a == b && i < j); }
+constexpr int kGather = 512;  // candidates that LDS holds; a chunk or group with more that reach the bound (many equal logits, the best
+                              // ones all in a few lanes) is walked K times instead
 
 // e^(x - m) for x <= m, by 2^y with y = (x - m) log2(e) in two parts
 DEV float exp_below(float x, float m) {
@@ -27,235 +26,328 @@ DEV float exp_below(float x, float m) {
   return __builtin_amdgcn_exp2f(fmaf(d, 1.4426950216293335f, d * 1.9259629911266175e-8f));
 }
 
-template <typename T> struct Quad;
-template <> struct Quad<float> {
+// 16 bytes of logits
+template <typename T> struct Piece;
+template <> struct Piece<float> {
   static constexpr int N = 4;
-  f32x4 v;
-  DEV float at(int i) const { return v[i]; }
-  DEV void put(int i, float x) { v[i] = x; }
+  static constexpr uint32_t kNone = 0xff800000u;  // -inf
+  u32x4 v;
+  DEV float at(int i) const { return __uint_as_float(v[i]); }
+  DEV void drop(int i, bool yes) { v[i] = yes ? kNone : v[i]; }
 };
-template <> struct Quad<bf16> {
+template <> struct Piece<bf16> {
   static constexpr int N = 8;
-  bf16x8 v;
-  DEV float at(int i) const { return (float)v[i]; }
-  DEV void put(int i, float x) { v[i] = (bf16)x; }
+  static constexpr uint32_t kNone = 0xff80ff80u;
+  u32x4 v;
+  DEV float at(int i) const { return __uint_as_float(i % 2 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16); }
+  DEV void drop(int i, bool yes) { v[i / 2] = yes ? (v[i / 2] & (i % 2 ? 0xffffu : 0xffff0000u)) | (kNone & (i % 2 ? 0xffff0000u : 0xffffu)) : v[i / 2]; }
 };
 
-// Q: 16-byte pieces of a thread
+// (value descending, token ascending) as the order of one number; -0 counts as 0
+DEV uint64_t logit_key(float v, int token) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~token;
+}
+DEV float key_logit(uint64_t k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+template <typename V>
+DEV V lane_value(V v, int lane) {  // a wave-uniform lane's value, without LDS
+  static_assert(sizeof(V) % 4 == 0, "whole words");
+  uint32_t w[sizeof(V) / 4];
+  __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(V) / 4; ++i) w[i] = __builtin_amdgcn_readlane(w[i], lane);
+  __builtin_memcpy(&v, w, sizeof(V));
+  return v;
+}
+
+// The K-th largest of 64 buckets' maxima, the same for every thread; mine: this thread's maximum, bucket = lane
+template <typename V>
+DEV V bound_of(V mine, int K, V (*all)[64], int* rank) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  all[wave][lane] = mine;
+  if (wave == 0) rank[lane] = 0;
+  __syncthreads();
+  V v = all[0][lane];
+#pragma unroll
+  for (int w = 1; w < kSelWaves; ++w) v = all[w][lane] > v ? all[w][lane] : v;
+  int n = 0;  // buckets before this one, a quarter of them per wave; of equal ones the lower lane is before
+#pragma unroll
+  for (int i = 0; i < 64 / kSelWaves; ++i) {
+    const int l = wave * (64 / kSelWaves) + i;
+    const V u = lane_value(v, l);
+    n += u > v || (u == v && l < lane) ? 1 : 0;
+  }
+  atomicAdd(&rank[lane], n);
+  __syncthreads();
+  const unsigned long long who = __ballot(rank[lane] == K - 1);
+  return lane_value(v, __ffsll(who) - 1);
+}
+
+// Q: 16-byte pieces of a thread.  A row is whole pieces at 16-byte addresses and the few elements before and behind them, which go
+// to the first threads of its first workgroup, one each.
 template <typename T, int Q>
-__global__ void __launch_bounds__(kSelThreads) beam_rows_kernel(BeamSelectParams p) {
-  constexpr int N = Quad<T>::N;
+__global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectParams p) {
+  constexpr int N = Piece<T>::N;
   __shared__ float s_max[kSelWaves], s_sum[kSelWaves];
-  __shared__ float b_val[kSelWaves][64];
-  __shared__ int b_idx[kSelWaves][64];
-  __shared__ float t_val;
-  __shared__ int t_idx, count;
-  __shared__ float g_val[kSelThreads * Q * N];
-  __shared__ int g_idx[kSelThreads * Q * N];
+  __shared__ float bucket[kSelWaves][64];
+  __shared__ int rank[64], count;
+  __shared__ uint64_t got[kGather];
   const int row = blockIdx.y, c = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
-  const int lo = c * p.chunk, hi = min(p.V, lo + p.chunk);
-  // pieces of 16 bytes at 16-byte addresses; `skew` elements of the first one belong to what is before the chunk
-  const int skew = (int)(reinterpret_cast<uintptr_t>(x + lo) % 16 / sizeof(T));
-  const int first = lo - skew;
-  Quad<T> q[Q];
+  const int head = min((int)(-reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)), p.V), pieces = (p.V - head) / N;
+  const int place = c * Q * kSelThreads + (int)threadIdx.x;  // of this thread's first piece; the others kSelThreads apart
+  Piece<T> q[Q];
+  float extra = -INFINITY;
+  int extra_at = -1;
   if (threadIdx.x == 0) count = 0;
-  float m = -INFINITY;
+  if (pieces > 0) {  // all requested before the first is used
 #pragma unroll
-  for (int k = 0; k < Q; ++k) {
-    const int e = first + (k * kSelThreads + threadIdx.x) * N;
-    if (e >= lo && e + N <= hi) {
-      q[k].v = ld_global<decltype(q[k].v)>(x + e);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) q[k].put(i, e + i >= lo && e + i < hi ? (float)x[e + i] : -INFINITY);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, q[k].at(i));
+    for (int k = 0; k < Q; ++k) q[k].v = ld_global<u32x4>(x + head + min(place + k * kSelThreads, pieces - 1) * N);
   }
-  m = wave_max(m);
-  if (lane == 0) s_max[wave] = m;
-  __syncthreads();
+  if (c == 0 && (int)threadIdx.x < p.V - pieces * N) {
+    extra_at = (int)threadIdx.x < head ? threadIdx.x : pieces * N + threadIdx.x;
+    extra = (float)x[extra_at];
+  }
+  if ((c + 1) * Q * kSelThreads > pieces) {  // what is past the row
 #pragma unroll
-  for (int w = 0; w < kSelWaves; ++w) m = fmaxf(m, s_max[w]);
-  const float ref = fmaxf(m, -3.4028234663852886e38f);  // a chunk of -inf alone sums to zero
-  float sum = 0.f;
-  float best = -INFINITY;
-  int bidx = 0x7fffffff - lane;  // lanes without a value keep places of their own
+    for (int k = 0; k < Q; ++k)
 #pragma unroll
-  for (int k = 0; k < Q; ++k) {
-    const int e = first + (k * kSelThreads + threadIdx.x) * N;
-    if (p.eos >= e && p.eos < e + N && p.eos >= lo && p.eos < hi) {  // the end token counts in the sum and is no candidate
+      for (int i = 0; i < 4; ++i) q[k].v[i] = place + k * kSelThreads < pieces ? q[k].v[i] : Piece<T>::kNone;
+  }
+  // the end token counts in the sum and is no candidate
+  float end = -INFINITY;
+  const int ahead = p.eos - head - place * N;  // elements from this thread's first one to it
+  if (p.eos >= 0) {
+    bool mine = extra_at == p.eos;
+    if (mine) extra = -INFINITY;
+    if (__any(ahead >= 0 && ahead < Q * kSelThreads * N)) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (e + i == p.eos) {
-          if (p.end_scores) p.end_logit[row] = q[k].at(i);
-          sum += exp_below(q[k].at(i), ref);
-          q[k].put(i, -INFINITY);
+      for (int k = 0; k < Q; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const bool here = ahead == k * kSelThreads * N + i && place + k * kSelThreads < pieces;
+          mine = mine || here;
+          q[k].drop(i, here);
         }
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float v = q[k].at(i);
-      sum += exp_below(v, ref);
-      if (v > best) best = v, bidx = e + i;
+    if (mine) {
+      end = (float)x[p.eos];
+      if (p.end_scores) p.end_logit[row] = end;
     }
   }
-  sum = wave_sum(sum);
-  if (lane == 0) s_sum[wave] = sum;
-  b_val[wave][lane] = best;
-  b_idx[wave][lane] = bidx;
-  __syncthreads();
-  if (wave == 0) {
-    for (int w = 1; w < kSelWaves; ++w)
-      if (before(b_val[w][lane], b_idx[w][lane], best, bidx)) best = b_val[w][lane], bidx = b_idx[w][lane];
-    int rank = 0;
-    for (int l = 0; l < 64; ++l) {
-      const float v = __shfl(best, l);
-      const int i = __shfl(bidx, l);
-      rank += before(v, i, best, bidx) ? 1 : 0;
-    }
-    if (rank == p.K - 1) t_val = best, t_idx = bidx;
-    if (lane == 0) {
-      float all = 0.f;
-      for (int w = 0; w < kSelWaves; ++w) all += s_sum[w];
-      p.stat[(size_t)row * p.chunks + c] = make_float2(ref, all);
-    }
-  }
-  __syncthreads();
-  const float tv = t_val;
-  const int ti = t_idx;
+  float most[Q], m = extra;
 #pragma unroll
   for (int k = 0; k < Q; ++k) {
-    const int e = first + (k * kSelThreads + threadIdx.x) * N;
+    most[k] = q[k].at(0);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float v = q[k].at(i);
-      if (v > -INFINITY && (v > tv || (v == tv && e + i <= ti))) {
-        const int at = atomicAdd(&count, 1);
-        g_val[at] = v;
-        g_idx[at] = e + i;
-      }
+    for (int i = 1; i < N; ++i) most[k] = fmaxf(most[k], q[k].at(i));
+    m = fmaxf(m, most[k]);
+  }
+  const float ref = fmaxf(fmaxf(m, end), -3.4028234663852886e38f);  // -inf alone sums to zero
+  float sum = exp_below(extra, ref) + exp_below(end, ref);
+#pragma unroll
+  for (int k = 0; k < Q; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += exp_below(q[k].at(i), ref);
+  const float top = wave_max(ref);
+  sum = wave_sum(sum * exp_below(ref, top));
+  if (lane == 0) s_max[wave] = top, s_sum[wave] = sum;
+  const float bound = bound_of(m, p.K, bucket, rank);
+  if (threadIdx.x == 0) {
+    float all = s_max[0], s = 0.f;
+#pragma unroll
+    for (int w = 1; w < kSelWaves; ++w) all = fmaxf(all, s_max[w]);
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) s += s_sum[w] * exp_below(s_max[w], all);
+    p.stat[(size_t)row * p.chunks + c] = make_float2(all, s);
+  }
+  // pieces that reach the bound are few: they are read again (from the caches), so that the registers need no index
+  auto gather = [&](float v, int token) {
+    if (v >= bound && v > -INFINITY && token != p.eos) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kGather) got[at] = logit_key(v, token);
     }
+  };
+  uint32_t hits = 0;
+#pragma unroll
+  for (int k = 0; k < Q; ++k) hits |= most[k] >= bound && most[k] > -INFINITY ? 1u << k : 0u;
+  if (extra_at >= 0) gather(extra, extra_at);
+  while (hits) {
+    const int token = head + (place + (__ffs(hits) - 1) * kSelThreads) * N;
+    hits &= hits - 1;
+    Piece<T> h;
+    h.v = ld_global<u32x4>(x + token);
+#pragma unroll
+    for (int i = 0; i < N; ++i) gather(h.at(i), token + i);
   }
   __syncthreads();
   const int n = count;
   float2* cand = p.cand + ((size_t)row * p.chunks + c) * p.K;
-  for (int a = threadIdx.x; a < n; a += kSelThreads) {
-    const float v = g_val[a];
-    const int i = g_idx[a];
-    int rank = 0;
-    for (int b = 0; b < n; ++b) rank += before(g_val[b], g_idx[b], v, i) ? 1 : 0;
-    if (rank < p.K) cand[rank] = make_float2(v, __int_as_float(i));
+  auto put = [&](int at, uint64_t key) { cand[at] = make_float2(key_logit(key), __int_as_float(~(int)(uint32_t)key)); };
+  if (n <= kGather) {
+    for (int a = threadIdx.x; a < n; a += kSelThreads) {
+      const uint64_t key = got[a];
+      int before = 0;
+#pragma unroll 8
+      for (int b = 0; b < n; ++b) before += got[b] > key ? 1 : 0;
+      if (before < p.K) put(before, key);
+    }
+  } else {
+    uint64_t prev = ~0ull;
+    for (int at = 0; at < p.K; ++at) {
+      uint64_t best = 0;
+      auto next = [&](float v, int token) {
+        const uint64_t key = logit_key(v, token);
+        if (v > -INFINITY && token != p.eos && key < prev && key > best) best = key;
+      };
+      if (extra_at >= 0) next(extra, extra_at);
+      for (int e = place; e < min(place + Q * kSelThreads, pieces); e += kSelThreads)
+        for (int i = 0; i < N; ++i) next((float)x[head + e * N + i], head + e * N + i);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) {
+        const uint64_t other = __shfl_xor((unsigned long long)best, o);
+        best = other > best ? other : best;
+      }
+      if (lane == 0) got[wave + kSelWaves * (at & 1)] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kSelWaves; ++w) best = max(best, got[w + kSelWaves * (at & 1)]);
+      if (threadIdx.x == 0) put(at, best);
+      prev = best;
+    }
   }
   for (int a = n + threadIdx.x; a < p.K; a += kSelThreads) cand[a] = make_float2(-INFINITY, __int_as_float(-1));
 }
 
 struct Pick {
   double s;
-  int row, token;  // row: beam of the group
+  int id;  // beam of the group * V + token
 };
-DEV bool before(const Pick& a, const Pick& b) {
-  return a.s > b.s || (a.s == b.s && (a.row < b.row || (a.row == b.row && a.token < b.token)));
-}
-DEV Pick shfl_pick(const Pick& a, int lane) { return Pick{__shfl(a.s, lane), __shfl(a.row, lane), __shfl(a.token, lane)}; }
-DEV Pick shfl_xor_pick(const Pick& a, int o) { return Pick{__shfl_xor(a.s, o), __shfl_xor(a.row, o), __shfl_xor(a.token, o)}; }
+DEV bool before(const Pick& a, const Pick& b) { return a.s > b.s || (a.s == b.s && a.id < b.id); }
 
 __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParams p) {
-  __shared__ double base[kBeamWidth], top[kBeamWidth];  // scores[row] - log(sum about `top`); NaN: the row offers nothing
-  __shared__ Pick bucket[kSelWaves][64], thr, got[kMergeCap];
-  __shared__ int count;
+  constexpr int kHeld = 4;                               // candidates of a thread that its registers hold
+  __shared__ double base[kBeamWidth];                    // scores[row] - log(sum about `top`); NaN: the row offers nothing
+  __shared__ float top[kBeamWidth];
+  __shared__ double bucket[kSelWaves][64];
+  __shared__ Pick gathered[2][kGather];
+  __shared__ int rank[64], count[2];
   const int g = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x == 0) count = 0;
-  for (int w = wave; w < p.width; w += kSelWaves) {
+  if (threadIdx.x == 0) count[0] = count[1] = 0;
+  // The chunks' lists are in order: their first `deep` places are looked at, the others only where the last of those reaches the
+  // bound.  Candidate e: place e / lists of list e % lists -- neighbouring threads look at different lists.
+  const int lists = p.width * p.chunks, deep = min(p.K, max(1, kHeld * kSelThreads / lists)), total = lists * deep;
+  const float2* cand = p.cand + (size_t)g * lists * p.K;
+  auto load = [&](int e) { return cand[(size_t)(e % lists) * p.K + e / lists]; };
+  float2 held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = load(min((int)threadIdx.x + i * kSelThreads, total - 1));
+  for (int w = threadIdx.x >> 4; w < p.width; w += kSelThreads / 16) {  // 16 lanes per row
     const float2* st = p.stat + (size_t)(g * p.width + w) * p.chunks;
+    const int l = threadIdx.x & 15;
     float m = -INFINITY;
-    for (int c = lane; c < p.chunks; c += 64) m = fmaxf(m, st[c].x);
-    m = wave_max(m);
+    for (int c = l; c < p.chunks; c += 16) m = fmaxf(m, st[c].x);
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     double sum = 0;
-    for (int c = lane; c < p.chunks; c += 64) sum += (double)st[c].y * exp((double)st[c].x - (double)m);
-    sum = wave_sum(sum);
-    if (lane == 0) {
+    for (int c = l; c < p.chunks; c += 16) sum += (double)st[c].y * exp((double)st[c].x - (double)m);
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    if (l == 0) {
       const float s = p.scores[g * p.width + w];
       const bool ok = s - s == 0.f && m - m == 0.f && sum - sum == 0. && sum > 0.;
-      base[w] = ok ? (double)s - log(sum) : __builtin_nan("");
+      const double b = ok ? (double)s - log(sum) : __builtin_nan("");
+      base[w] = b;
       top[w] = m;
-      if (p.end_scores) {
-        const float e = p.end_logit[g * p.width + w];
-        p.end_scores[g * p.width + w] = ok ? (float)(base[w] + ((double)e - (double)m)) : -INFINITY;
-      }
+      if (p.end_scores) p.end_scores[g * p.width + w] = ok ? (float)(b + ((double)p.end_logit[g * p.width + w] - (double)m)) : -INFINITY;
     }
   }
   __syncthreads();
-  const int lists = p.width * p.chunks, total = lists * p.K;
-  const float2* cand = p.cand + (size_t)g * total;
-  // candidate e: list e % lists, place e / lists -- neighbouring threads look at different lists
-  auto pick_of = [&](int e) {
-    const int l = e % lists, w = l / p.chunks;
-    const float2 c = cand[(size_t)l * p.K + e / lists];
+  auto pick_of = [&](int list, float2 c) {
+    const int w = list / p.chunks;
     const double b = base[w];
-    Pick r{-INFINITY, 0x7fffffff, e};
-    if (c.x > -INFINITY && b == b) r = Pick{b + ((double)c.x - top[w]), w, __float_as_int(c.y)};
+    Pick r{-INFINITY, 0x7fffffff};
+    if (c.x > -INFINITY && b == b) r = Pick{b + ((double)c.x - (double)top[w]), w * p.V + __float_as_int(c.y)};
     return r;
   };
-  Pick best{-INFINITY, 0x7fffffff, 0x7fffffff - (int)threadIdx.x};
-  for (int e = threadIdx.x; e < total; e += kSelThreads) {
-    const Pick c = pick_of(e);
-    if (before(c, best)) best = c;
-  }
-  bucket[wave][lane] = best;
-  __syncthreads();
-  if (wave == 0) {
-    for (int w = 1; w < kSelWaves; ++w)
-      if (before(bucket[w][lane], best)) best = bucket[w][lane];
-    int rank = 0;
-    for (int l = 0; l < 64; ++l) rank += before(shfl_pick(best, l), best) ? 1 : 0;
-    if (rank == p.K - 1) thr = best;
-  }
-  __syncthreads();
-  const Pick t = thr;
-  for (int e = threadIdx.x; e < total; e += kSelThreads) {
-    const Pick c = pick_of(e);
-    if (c.s > -INFINITY && !before(t, c)) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kMergeCap) got[at] = c;
+  // the looked-at candidates of this thread, those in registers first
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int e = threadIdx.x + i * kSelThreads;
+      if (e < total) f(pick_of(e % lists, held[i]), e);
     }
-  }
+    for (int e = threadIdx.x + kHeld * kSelThreads; e < total; e += kSelThreads) f(pick_of(e % lists, load(e)), e);
+  };
+  double best = -INFINITY;
+  each([&](const Pick& c, int) { best = c.s > best ? c.s : best; });
+  const double bound = bound_of(best, p.K, bucket, rank);
+  auto gather = [&](const Pick& c) {
+    const bool in = c.s >= bound && c.s > -INFINITY;
+    if (in) {
+      const int at = atomicAdd(&count[0], 1);
+      if (at < kGather) gathered[0][at] = c;
+    }
+    return in;
+  };
+  if (best >= bound)
+    each([&](const Pick& c, int e) {
+      if (gather(c) && e / lists == deep - 1)
+        for (int at = deep; at < p.K && gather(pick_of(e % lists, cand[(size_t)(e % lists) * p.K + at])); ++at) {
+        }
+    });
   __syncthreads();
-  const int n = count;
+  int n = count[0];
+  Pick* got = gathered[0];
+  if (n > 2 * p.K && n <= kGather) {
+    // A row far ahead has its best in few lists, and the lists' maxima say little: the same bound once more among the gathered
+    // ones, which lie in no order.
+    best = -INFINITY;
+    for (int a = threadIdx.x; a < n; a += kSelThreads) best = got[a].s > best ? got[a].s : best;
+    const double nearer = bound_of(best, p.K, bucket, rank);
+    for (int a = threadIdx.x; a < n; a += kSelThreads)
+      if (got[a].s >= nearer) gathered[1][atomicAdd(&count[1], 1)] = got[a];
+    __syncthreads();
+    n = count[1];
+    got = gathered[1];
+  }
   auto put = [&](int at, const Pick& c) {
     p.out_scores[(size_t)g * p.K + at] = (float)c.s;
-    p.out_rows[(size_t)g * p.K + at] = g * p.width + c.row;
-    p.out_tokens[(size_t)g * p.K + at] = c.token;
+    p.out_rows[(size_t)g * p.K + at] = g * p.width + c.id / p.V;
+    p.out_tokens[(size_t)g * p.K + at] = c.id % p.V;
   };
-  if (n <= kMergeCap) {
+  if (n <= kGather) {
     for (int a = threadIdx.x; a < n; a += kSelThreads) {
       const Pick c = got[a];
-      int rank = 0;
-      for (int b = 0; b < n; ++b) rank += before(got[b], c) ? 1 : 0;
-      if (rank < p.K) put(rank, c);
+      int at = 0;
+#pragma unroll 8
+      for (int b = 0; b < n; ++b) at += before(got[b], c) ? 1 : 0;
+      if (at < p.K) put(at, c);
     }
   } else {
-    // more than LDS holds (the best ones all in a few lanes' lists): one place after another
-    Pick prev{INFINITY, -1, -1};
+    Pick prev{INFINITY, -1};
     for (int at = 0; at < p.K; ++at) {
-      Pick b{-INFINITY, 0x7fffffff, 0x7fffffff};
-      for (int e = threadIdx.x; e < total; e += kSelThreads) {
-        const Pick c = pick_of(e);
+      Pick b{-INFINITY, 0x7fffffff};
+      for (int e = threadIdx.x; e < lists * p.K; e += kSelThreads) {
+        const Pick c = pick_of(e / p.K, cand[e]);
         if (before(prev, c) && before(c, b)) b = c;
       }
+#pragma unroll
       for (int o = 32; o >= 1; o >>= 1) {
-        const Pick c = shfl_xor_pick(b, o);
+        const Pick c{__shfl_xor(b.s, o), __shfl_xor(b.id, o)};
         if (before(c, b)) b = c;
       }
+      if (lane == 0) got[wave + kSelWaves * (at & 1)] = b;
       __syncthreads();
-      if (lane == 0) bucket[wave][0] = b;
-      __syncthreads();
-      b = bucket[0][0];
-      for (int w = 1; w < kSelWaves; ++w)
-        if (before(bucket[w][0], b)) b = bucket[w][0];
+#pragma unroll
+      for (int w = 0; w < kSelWaves; ++w)
+        if (before(got[w + kSelWaves * (at & 1)], b)) b = got[w + kSelWaves * (at & 1)];
       if (threadIdx.x == 0) put(at, b);
       prev = b;
     }
@@ -270,12 +362,10 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
 template <typename T>
 hipError_t launch_rows(const BeamSelectParams& p, hipStream_t st) {
   const dim3 grid(p.chunks, p.rows), block(kSelThreads);
-  constexpr int N = Quad<T>::N, kPiece = kSelThreads * N;
-  const bool whole = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld % N == 0 && p.chunk % N == 0;
-  const int q = (p.chunk + (whole ? 0 : N - 1) + kPiece - 1) / kPiece;  // a chunk that begins inside a piece needs one more
-  if (q <= 1) hipLaunchKernelGGL((beam_rows_kernel<T, 1>), grid, block, 0, st, p);
-  else if (q <= 2) hipLaunchKernelGGL((beam_rows_kernel<T, 2>), grid, block, 0, st, p);
-  else if (q <= 4 && N == 4) hipLaunchKernelGGL((beam_rows_kernel<T, 4>), grid, block, 0, st, p);
+  if (p.pieces == 1) hipLaunchKernelGGL((beam_rows_kernel<T, 1>), grid, block, 0, st, p);
+  else if (p.pieces == 2) hipLaunchKernelGGL((beam_rows_kernel<T, 2>), grid, block, 0, st, p);
+  else if (p.pieces == 4) hipLaunchKernelGGL((beam_rows_kernel<T, 4>), grid, block, 0, st, p);
+  else if (p.pieces == 8) hipLaunchKernelGGL((beam_rows_kernel<T, 8>), grid, block, 0, st, p);
   else return hipErrorInvalidValue;
   return hipGetLastError();
 }
@@ -283,20 +373,20 @@ hipError_t launch_rows(const BeamSelectParams& p, hipStream_t st) {
 }  // namespace
 }  // namespace dsse
 
-// Vocabulary of a workgroup: as much as its registers hold, less while that leaves CUs empty
-extern "C" int dsse_beam_chunk(int rows, int V, int f32, int whole) {
-  const int n = f32 ? 4 : 8;
-  for (int q = f32 ? 4 : 2; q >= 1; q /= 2) {
-    const int chunk = q * dsse::kSelThreads * n - (whole ? 0 : n);
-    if (q == 1 || (int64_t)rows * ((V + chunk - 1) / chunk) >= 512) return chunk;
+// Pieces of a thread: as many as its registers hold, fewer while that leaves CUs empty
+extern "C" void dsse_beam_plan_rows(dsse::BeamSelectParams* p) {
+  const int n = p->f32 ? 4 : 8, row = (p->V + n - 1) / n;
+  for (p->pieces = 8;; p->pieces /= 2) {
+    const int chunk = p->pieces * dsse::kSelThreads;
+    p->chunks = (row + chunk - 1) / chunk;
+    if (p->pieces == 1 || (int64_t)p->rows * p->chunks >= 512) return;
   }
-  return 1;
 }
 
 extern "C" hipError_t dsse_beam_select(const dsse::BeamSelectParams* p, hipStream_t st) {
   using namespace dsse;
   if (p->width < 1 || p->width > kBeamWidth || p->K < 1 || p->K > kBeamKeep || p->rows % p->width || p->rows > 65535 || p->V < 1 ||
-      p->chunk < 1 || (int64_t)p->chunk * p->chunks < p->V)
+      (int64_t)p->pieces * kSelThreads * p->chunks * (p->f32 ? 4 : 8) < p->V)
     return hipErrorInvalidValue;
   if (p->rows == 0) return hipSuccess;
   const hipError_t e = p->f32 ? launch_rows<float>(*p, st) : launch_rows<bf16>(*p, st);

@@ -74,9 +74,7 @@ void beam_select(const Tensor& logits, const Tensor& scores, Tensor& out_scores,
   p.ld = logits.size(0) == 1 ? V : logits.stride(0);
   p.f32 = logits.scalar_type() == at::kFloat ? 1 : 0;
   p.rows = (int)logits.size(0), p.width = (int)scores.size(1), p.V = (int)V, p.K = (int)K, p.eos = (int)eos_id;
-  const bool whole = aligned16(p.logits) && p.ld % (p.f32 ? 4 : 8) == 0;
-  p.chunk = dsse_beam_chunk(p.rows, p.V, p.f32, whole ? 1 : 0);
-  p.chunks = (p.V + p.chunk - 1) / p.chunk;
+  dsse_beam_plan_rows(&p);
   // [statistics | candidates | end logits]
   const int64_t parts = (int64_t)p.rows * p.chunks;
   Tensor work = at::empty({2 * parts * (1 + K) + p.rows}, scores.options());
