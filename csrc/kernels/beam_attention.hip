@@ -1,223 +1,342 @@
 // Attention of one new token per beam over the paged cache, for requests whose beams share pages (layouts of attention.hip).
 //
 // A group's leading `shared` pages are the same in all of its tables.  They are read once for the group: the columns of the score
-// tile Sᵀ = K Qᵀ are (beam, q head) pairs, so a page's K and V fragments feed every beam.  The pages behind them are read per
-// slot.  Both walks are cut over their length, and a second launch joins the parts of a (slot, q head):
+// tile Sᵀ = K Qᵀ are (beam, q head) pairs, so a page's K and V feed every beam.  The pages behind them are read per slot.  Both walks
+// are cut over their length, and a second launch joins the parts of a (slot, q head):
 //
-//   work items  x < col_blocks * ns: the shared keys of group z, part x % ns, columns of block x / ns
-//               else               : a slot's own keys, part (x - col_blocks * ns) % no
+//   work items  x < groups * col_blocks * ns: the shared keys of a group, a block of columns, one of ns parts
+//               else                        : a slot's own keys, one of no parts
 //
-// Statistics and sums in fp32; scores in base 2 with the scale folded in; bf16 products as in paged_attention.
+// T = 1 (up to 16 columns): four waves take the pages in turn, straight to registers, and join their sums in LDS.
+// T = 2, 4, 8: a wave per column tile; the pages pass through LDS once for all waves, filled by LDS-DMA kRing - 1 pages ahead.  A
+// page costs 16 KB from memory and T tiles' products, so what bounds it is memory; the ring keeps it busy with one wave per SIMD.
+//
+// Statistics and sums in fp32; scores in base 2 with the scale folded in; weights rounded to bf16 for the second product, as in
+// paged_attention.
 #include "api_beams.h"
+#include "lds_dma.h"
+
+#include <atomic>
 
 namespace dsse {
 namespace {
 
 constexpr int kPg = 32;
 constexpr int kDim = 128;
-constexpr int kBeamWaves = 4;
-constexpr float kLow = -1e30f;  // a finite start: fully masked columns stay finite and sum to zero
+constexpr int kHalf = kPg * kDim * 2;  // bytes of a page's keys, or of its values
+constexpr int kRing = 5;               // pages in LDS; two workgroups of a CU fill its 160 KB
+constexpr float kLow = -1e30f;         // a finite start: fully masked columns stay finite and sum to zero
 
-// shared pages of a group that every live beam has whole; live: the first live slot, -1 if none
+constexpr int waves_of(int T) { return T == 1 ? 4 : T; }
+
+// Shared pages of a group that every live beam has whole; live: the first live slot, -1 if none
 DEV int group_pages(const BeamAttnParams& p, int g, int& live) {
-  int pages = min(p.shared[g], p.max_blocks);
-  live = -1;
-  for (int w = 0; w < p.width; ++w) {
-    const int s = g * p.width + w, n = p.ctx_len[s];
-    if (n <= 0) continue;
-    if (live < 0) live = s;
-    pages = min(pages, n / kPg);
-  }
-  return live < 0 ? 0 : max(pages, 0);
+  const int w = threadIdx.x & 63;
+  const int n = w < p.width ? p.ctx_len[g * p.width + w] : 0;
+  const unsigned long long mask = __ballot(n > 0);
+  int pages = n > 0 ? n / kPg : 0x7fffffff;
+#pragma unroll
+  for (int o = 1; o < kBeamWidth; o <<= 1) pages = min(pages, __shfl_xor(pages, o));
+  pages = __builtin_amdgcn_readfirstlane(pages);
+  live = __builtin_amdgcn_readfirstlane(mask ? g * p.width + __ffsll(mask) - 1 : -1);
+  return __builtin_amdgcn_readfirstlane(mask ? max(0, min(min(pages, p.shared[g]), p.max_blocks)) : 0);
 }
 
-// Keys [kPg pb, min(kPg pe, limit)) of a table row for CT tiles of 16 columns, by the waves of a workgroup; leaves a wave's sums
-template <int CT>
-DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int limit, const bf16x8 (&qf)[CT][4], f32x4 (&o)[CT][8],
-              float (&m)[CT], float (&l)[CT]) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = threadIdx.x >> 6;
-  for (int pg = pb + kw; pg < pe; pg += kBeamWaves) {
-    int page = __builtin_amdgcn_readfirstlane(bt[pg]);
-    page = (unsigned)page < (unsigned)p.num_blocks ? page : 0;  // an id that is no page reads page 0, not past the cache
-    const bf16* kp = p.k_cache + ((size_t)page * p.hkv + h) * kPg * kDim;
-    const bf16* vp = p.v_cache + ((size_t)page * p.hkv + h) * kDim * kPg;
+// Entry `pg` of a table row: a wave-uniform scalar load, which does not wait for the vector loads in flight.  (The tables are
+// read-only for the kernel.)
+DEV int entry(const int* bt, int pg) {
+  return ((const __attribute__((address_space(4))) int*)bt)[__builtin_amdgcn_readfirstlane(pg)];
+}
+// An entry that is no page reads page 0, not past the cache
+DEV int page_of(const BeamAttnParams& p, int entry) { return (unsigned)entry < (unsigned)p.num_blocks ? entry : 0; }
+
+struct Column {  // 16 columns' running sums of a wave: lane (r, g) holds head dims 16 dt + 4 g + i of column r
+  f32x4 o[8];
+  float m, l;
+  DEV void clear() {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = kLow;
+    l = 0.f;
+  }
+  // The weights of a page's scores (keys 4g + i and 16 + 4g + i of column r), as the second product's operand
+  DEV bf16x8 weigh(const f32x4& s0, const f32x4& s1, float scale, int left) {
+    float s[8], top = -INFINITY;
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = (i < 4 ? s0[i] : s1[i - 4]) * scale;
+    if (left < kPg) {  // keys of the page past the sequence
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = (i < 4 ? 4 * g + i : 12 + 4 * g + i) < left ? s[i] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i]);
+    const float now = fmaxf(m, rows4_max(top));
+    if (__any(now > m)) {  // after the first pages a maximum moves rarely
+      const float by = __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= by;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) o[dt] *= by;
+    }
+    bf16x8 w;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float e = __builtin_amdgcn_exp2f(s[i] - m);
+      sum += e;
+      w[i] = f2bf(e);
+    }
+    l += sum;
+    return w;
+  }
+};
+
+// What a page holds past the sequence is not read as a number: 0 * NaN would reach the sums
+DEV void blank_values(bf16x8 (&vf)[8], int left) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool in = (j < 4 ? 4 * g + j : 12 + 4 * g + j) < left;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) vf[dt][j] = in ? vf[dt][j] : (bf16)0.f;
+  }
+}
+
+// Keys of pages [pb, pe) up to `limit`, for 16 columns, pages in turn to NW waves
+template <int NW>
+DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int limit, int row, Column& c) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  bf16x8 qf[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) qf[k] = row >= 0 ? ld_bf16x8(p.q + (size_t)row * kDim + 32 * k + 8 * g) : zero_bf16x8();
+  c.clear();
+  int id = entry(bt, min(pb + kw, pe - 1));
+  for (int pg = pb + kw; pg < pe; pg += NW) {
+    const size_t at = ((size_t)page_of(p, id) * p.hkv + h) * kPg * kDim;
+    id = entry(bt, min(pg + NW, pe - 1));  // the next one is on its way while this page is computed
+    const bf16 *kp = p.k_cache + at, *vp = p.v_cache + at;
     bf16x8 k0[4], k1[4], vf[8];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      k0[s] = ld_once<bf16x8>(kp + (size_t)r * kDim + 32 * s + 8 * g);
-      k1[s] = ld_once<bf16x8>(kp + (size_t)(16 + r) * kDim + 32 * s + 8 * g);
+      k0[s] = ld_once<bf16x8>(kp + r * kDim + 32 * s + 8 * g);
+      k1[s] = ld_once<bf16x8>(kp + (16 + r) * kDim + 32 * s + 8 * g);
     }
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) vf[dt] = ld_once<bf16x8>(vp + (size_t)(16 * dt + r) * kPg + 8 * g);
-    const int kb = pg * kPg;
-    const bool part = kb + kPg > limit;
-    if (part) {  // what a page holds past the sequence is not read as a number: 0 * NaN would reach the sums
+    for (int dt = 0; dt < 8; ++dt) vf[dt] = ld_once<bf16x8>(vp + (16 * dt + r) * kPg + 8 * g);
+    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = kb + (j < 4 ? 4 * g + j : 12 + 4 * g + j) < limit;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) vf[dt][j] = in ? vf[dt][j] : (bf16)0.f;
-      }
+    for (int s = 0; s < 4; ++s) {
+      s0 = mfma16x16x32(k0[s], qf[s], s0);
+      s1 = mfma16x16x32(k1[s], qf[s], s1);
     }
+    const int left = limit - pg * kPg;
+    const bf16x8 w = c.weigh(s0, s1, p.scale_log2, left);
+    if (left < kPg) blank_values(vf, left);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        s0 = mfma16x16x32(k0[s], qf[ct][s], s0);
-        s1 = mfma16x16x32(k1[s], qf[ct][s], s1);
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // keys kb + 4g + i and kb + 16 + 4g + i
-        s0[i] = !part || kb + 4 * g + i < limit ? s0[i] * p.scale_log2 : -INFINITY;
-        s1[i] = !part || kb + 16 + 4 * g + i < limit ? s1[i] * p.scale_log2 : -INFINITY;
-        top = fmaxf(top, fmaxf(s0[i], s1[i]));
-      }
-      top = rows4_max(top);
-      const float now = fmaxf(m[ct], top), alpha = exp2f(m[ct] - now);
-      m[ct] = now;
-      bf16x8 pf;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e0 = exp2f(s0[i] - now), e1 = exp2f(s1[i] - now);
-        sum += e0 + e1;
-        pf[i] = f2bf(e0);  // bf16 weights, as the values they meet; the sum above keeps 32 bits
-        pf[4 + i] = f2bf(e1);
-      }
-      l[ct] = l[ct] * alpha + sum;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32(vf[dt], pf, o[ct][dt] * alpha);
-    }
+    for (int dt = 0; dt < 8; ++dt) c.o[dt] = mfma16x16x32(vf[dt], w, c.o[dt]);
   }
 }
 
-struct MergeLds {
-  float o[kBeamWaves][32][64];
-  float m[kBeamWaves][16], l[kBeamWaves][16];
-};
+// The same for T column tiles, one per wave: whole pages [pb, pe) through LDS
+template <int T>
+DEV void walk_tiles(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int row, Column& c, char* smem) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // head dims of a k-step: 32 g + 8 s .. + 7 of both operands
+  bf16x8 qf[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) qf[s] = row >= 0 ? ld_bf16x8(p.q + (size_t)row * kDim + 32 * g + 8 * s) : zero_bf16x8();
+#pragma unroll
+  for (int s = 0; s < 4; ++s) asm volatile("" ::"v"(qf[s]));  // their wait is here, not behind the DMAs of the loop
+  c.clear();
+  // A page is 16 instructions of 1 KiB, a wave's all keys or all values.  Keys: 4 rows of 16 pieces, piece ^ swz(row); values: 16
+  // rows d of 4 pieces, piece ^ vswz(row): the swizzles sit on the source address and make the fragment reads free of conflicts.
+  constexpr int IPW = 16 / T;
+  auto vswz = [](int row) { return (4 - (row >> 2)) & 3; };
+  const bool keys = wave * IPW < 8;
+  uint32_t from[IPW];
+#pragma unroll
+  for (int i = 0; i < IPW; ++i) {
+    const int n = (wave * IPW + i) & 7;
+    from[i] = n * 1024 + (keys ? (lane >> 4) * 256 + (((lane & 15) ^ swz(4 * (n & 3) + (lane >> 4))) << 4)
+                               : (lane >> 2) * 64 + (((lane & 3) ^ vswz(lane >> 2)) << 4));
+  }
+  const bf16* mine = (keys ? p.k_cache : p.v_cache) + (size_t)h * kPg * kDim;
+  int id = entry(bt, pb), next = pb, slot_in = 0;
+  auto issue = [&]() {  // a page past the last lands as zeros, without traffic, so that every step issues as many
+    const __amdgpu_buffer_rsrc_t src = make_rsrc(mine + (size_t)page_of(p, id) * p.hkv * kPg * kDim, next < pe ? kHalf : 0);
+    ++next;
+    id = entry(bt, min(next, pe - 1));
+    char* to = smem + slot_in * 2 * kHalf + wave * IPW * 1024;
+    slot_in = slot_in + 1 == kRing ? 0 : slot_in + 1;
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) lds_dma<kAuxNT>(src, to + i * 1024, from[i]);
+  };
+  int kofs[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) kofs[s] = r * 256 + (((4 * g + s) ^ swz(r)) << 4);
+  const int vofs = kHalf + r * 64 + ((g ^ vswz(r)) << 4);
+  for (int i = 0; i < kRing - 1; ++i) issue();
+  int slot = 0;
+  for (int pg = pb; pg < pe; ++pg) {
+    // this page has landed in every wave's share, and every wave has read the page whose slot is filled next
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kRing - 2) * IPW) : "memory");
+    issue();
+    const char* at = smem + slot * 2 * kHalf;
+    slot = slot + 1 == kRing ? 0 : slot + 1;
+    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+    bf16x8 k0[4], k1[4], vf[8];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      k0[s] = *reinterpret_cast<const bf16x8*>(at + kofs[s]);
+      k1[s] = *reinterpret_cast<const bf16x8*>(at + 4096 + kofs[s]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) vf[dt] = *reinterpret_cast<const bf16x8*>(at + dt * 1024 + vofs);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      s0 = mfma16x16x32(k0[s], qf[s], s0);
+      s1 = mfma16x16x32(k1[s], qf[s], s1);
+    }
+    const bf16x8 w = c.weigh(s0, s1, p.scale_log2, kPg);
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) c.o[dt] = mfma16x16x32(vf[dt], w, c.o[dt]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way into LDS when the workgroup ends
+}
 
-// Joins the waves' sums of one column tile and leaves them as part z of the columns' (slot, head).  row: column r's
-// slot * hq + head, or -1.  Wave kw writes the head dims 32 kw .. 32 kw + 31.
-DEV void leave(const BeamAttnParams& p, MergeLds& lds, const f32x4 (&o)[8], float m, float l, int row, int z) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = threadIdx.x >> 6;
-  l = rows4_sum(l);
-  __syncthreads();
+// A column tile's sums as part z of the columns' rows (slot * hq + head, -1: no column)
+DEV void leave(const BeamAttnParams& p, const Column& c, int row, int z) {
+  const int g = (threadIdx.x & 63) >> 4, np = p.ns + p.no;
+  const float l = rows4_sum(c.l);
+  if (row < 0) return;
+  float* po = p.part_o + ((size_t)row * np + z) * kDim + 4 * g;
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = c.o[dt];
+  if (g == 0) p.part_ml[(size_t)row * np + z] = make_float2(c.m, l);
+}
+
+// The same for waves that split the keys of one column tile: joined in LDS, wave kw the head dims 128 kw / NW ..
+template <int NW>
+DEV void leave_joined(const BeamAttnParams& p, const Column& c, int row, int z, char* smem) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = threadIdx.x >> 6, np = p.ns + p.no;
+  float* o = reinterpret_cast<float*>(smem);   // [NW][32][64]
+  float* ms = o + NW * 32 * 64;                // [NW][16]
+  float* ls = ms + NW * 16;
+  const float own = rows4_sum(c.l);
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds.o[kw][dt * 4 + i][lane] = o[dt][i];
-  if (g == 0) lds.m[kw][r] = m, lds.l[kw][r] = l;
+    for (int i = 0; i < 4; ++i) o[(kw * 32 + dt * 4 + i) * 64 + lane] = c.o[dt][i];
+  if (g == 0) ms[kw * 16 + r] = c.m, ls[kw * 16 + r] = own;
   __syncthreads();
-  float top = lds.m[0][r];
+  float top = ms[r];
 #pragma unroll
-  for (int v = 1; v < kBeamWaves; ++v) top = fmaxf(top, lds.m[v][r]);
-  float w[kBeamWaves], sum = 0.f;
+  for (int v = 1; v < NW; ++v) top = fmaxf(top, ms[v * 16 + r]);
+  float w[NW], sum = 0.f;
 #pragma unroll
-  for (int v = 0; v < kBeamWaves; ++v) {
-    w[v] = exp2f(lds.m[v][r] - top);
-    sum += lds.l[v][r] * w[v];
+  for (int v = 0; v < NW; ++v) {
+    w[v] = __builtin_amdgcn_exp2f(ms[v * 16 + r] - top);
+    sum += ls[v * 16 + r] * w[v];
   }
   if (row < 0) return;
-  const int np = p.ns + p.no;
-  float* po = p.part_o + ((size_t)row * np + z) * kDim;
+  float* po = p.part_o + ((size_t)row * np + z) * kDim + 4 * g;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int dt = 2 * kw + t;
+  for (int t = 0; t < 8 / NW; ++t) {
+    const int dt = kw * (8 / NW) + t;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < kBeamWaves; ++v)
+    for (int v = 0; v < NW; ++v)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] += lds.o[v][dt * 4 + i][lane] * w[v];
-    *reinterpret_cast<f32x4*>(po + 16 * dt + 4 * g) = a;
+      for (int i = 0; i < 4; ++i) a[i] += o[(v * 32 + dt * 4 + i) * 64 + lane] * w[v];
+    *reinterpret_cast<f32x4*>(po + 16 * dt) = a;
   }
   if (kw == 0 && g == 0) p.part_ml[(size_t)row * np + z] = make_float2(top, sum);
 }
 
-template <int CT>
-__global__ void __launch_bounds__(64 * kBeamWaves) beam_attention_kernel(BeamAttnParams p) {
-  __shared__ MergeLds lds;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+// Pages [first, second) of part z of n: at least `least` pages a part, the rest empty
+DEV int2 part_of(int pages, int n, int z, int least) {
+  const int per = max((pages + n - 1) / n, least), pb = min(pages, z * per);
+  return make_int2(pb, min(pages, pb + per));
+}
+
+template <int T>
+__global__ void __launch_bounds__(64 * waves_of(T), 2) beam_attention_kernel(BeamAttnParams p) {
+  constexpr int NW = waves_of(T);
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63, r = lane & 15;
   const int h = blockIdx.y, np = p.ns + p.no;
-  const int groups = p.slots / p.width, nshared = groups * p.col_blocks * p.ns;
+  const int nshared = p.slots / p.width * p.col_blocks * p.ns;
+  int live;
+  Column c;
   if ((int)blockIdx.x < nshared) {
     const int z = blockIdx.x % p.ns, cb = blockIdx.x / p.ns % p.col_blocks, gr = blockIdx.x / (p.ns * p.col_blocks);
-    int live;
-    const int pages = group_pages(p, gr, live);
-    int row[CT];
-    bf16x8 qf[CT][4];
-    f32x4 o[CT][8];
-    float m[CT], l[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int c = (cb * CT + ct) * 16 + r, w = c / p.group, s = gr * p.width + w;
-      const bool in = w < p.width && p.ctx_len[s] > 0;
-      row[ct] = in ? s * p.hq + h * p.group + c % p.group : -1;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) qf[ct][k] = in ? ld_bf16x8(p.q + (size_t)row[ct] * kDim + 32 * k + 8 * g) : zero_bf16x8();
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      m[ct] = kLow;
-      l[ct] = 0.f;
-    }
-    const int per = (pages + p.ns - 1) / p.ns, pb = min(pages, z * per), pe = min(pages, pb + per);
-    if (pb >= pe) {  // nothing to read: the parts say so
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        if (threadIdx.x < 16 && row[ct] >= 0) p.part_ml[(size_t)row[ct] * np + z] = make_float2(kLow, 0.f);
+    const int2 part = part_of(group_pages(p, gr, live), p.ns, z, 4);
+    const int at = (cb * T + (T == 1 ? 0 : threadIdx.x >> 6)) * 16 + r, w = at / p.group, s = gr * p.width + w;
+    const int row = w < p.width && p.ctx_len[s] > 0 ? s * p.hq + h * p.group + at % p.group : -1;
+    if (part.x >= part.y) {  // nothing to read: the part says so
+      if (lane < 16 && row >= 0) p.part_ml[(size_t)row * np + z] = make_float2(kLow, 0.f);
       return;
     }
-    walk<CT>(p, p.block_tables + (size_t)live * p.max_blocks, h, pb, pe, pe * kPg, qf, o, m, l);
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) leave(p, lds, o[ct], m[ct], l[ct], row[ct], z);
+    const int* bt = p.block_tables + (size_t)live * p.max_blocks;
+    if constexpr (T == 1) {
+      walk<NW>(p, bt, h, part.x, part.y, part.y * kPg, row, c);
+      leave_joined<NW>(p, c, row, z, smem);
+    } else {
+      walk_tiles<T>(p, bt, h, part.x, part.y, row, c, smem);
+      leave(p, c, row, z);
+    }
   } else {
     const int x = blockIdx.x - nshared, z = x % p.no, s = x / p.no;
     const int n = p.ctx_len[s];
     if (n <= 0) return;
-    int live;
     const int skip = group_pages(p, s / p.width, live);
-    const int pages = min((n + kPg - 1) / kPg, p.max_blocks) - skip;
+    const int2 part = part_of(min((n + kPg - 1) / kPg, p.max_blocks) - skip, p.no, z, NW);
     const int row = r < p.group ? s * p.hq + h * p.group + r : -1;
-    const int per = (pages + p.no - 1) / p.no, pb = min(pages, z * per), pe = min(pages, pb + per);
-    if (pb >= pe) {
+    if (part.x >= part.y) {
       if (threadIdx.x < 16 && row >= 0) p.part_ml[(size_t)row * np + p.ns + z] = make_float2(kLow, 0.f);
       return;
     }
-    bf16x8 qf[1][4];
-    f32x4 o[1][8];
-    float m[1] = {kLow}, l[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) qf[0][k] = row >= 0 ? ld_bf16x8(p.q + (size_t)row * kDim + 32 * k + 8 * g) : zero_bf16x8();
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) o[0][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    walk<1>(p, p.block_tables + (size_t)s * p.max_blocks, h, skip + pb, skip + pe, n, qf, o, m, l);
-    leave(p, lds, o[0], m[0], l[0], row, p.ns + z);
+    walk<NW>(p, p.block_tables + (size_t)s * p.max_blocks, h, skip + part.x, skip + part.y, n, row, c);
+    leave_joined<NW>(p, c, row, p.ns + z, smem);
   }
 }
 
-// one wave per (slot, q head): lane z holds part z's statistics, then every lane two head dims
+// One wave per (slot, q head): lane z holds part z's statistics; then the parts that have keys, two at a time (a half wave each, four
+// head dims a lane), as many in flight as the loop is unrolled
 __global__ void __launch_bounds__(256) beam_join_kernel(BeamAttnParams p) {
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.slots * p.hq || p.ctx_len[row / p.hq] <= 0) return;
   const int np = p.ns + p.no;
   float2 ml = make_float2(kLow, 0.f);
   if (lane < np) ml = p.part_ml[(size_t)row * np + lane];
-  const float top = wave_max(ml.x), w = exp2f(ml.x - top);
+  const float top = wave_max(ml.x), w = __builtin_amdgcn_exp2f(ml.x - top);
   const float sum = wave_sum(ml.y * w);
-  const float* po = p.part_o + (size_t)row * np * kDim + 2 * lane;
-  float a = 0.f, b = 0.f;
-  for (int z = 0; z < np; ++z) {
-    if (__shfl(ml.y, z) == 0.f) continue;  // a part without keys has left no sums
-    const float wz = __shfl(w, z);
-    const f32x2 v = *reinterpret_cast<const f32x2*>(po + (size_t)z * kDim);
-    a += v[0] * wz;
-    b += v[1] * wz;
+  unsigned long long mask = __ballot(ml.x > kLow);  // a part without keys has left no sums
+  const float* po = p.part_o + (size_t)row * np * kDim + 4 * (lane & 31);
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  while (mask) {
+    f32x4 v[4];
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int z0 = mask ? __ffsll(mask) - 1 : 64;
+      mask &= mask - 1;
+      const int z1 = mask ? __ffsll(mask) - 1 : 64;
+      mask &= mask - 1;
+      const int z = lane < 32 ? z0 : z1;
+      const float by = __shfl(w, z & 63);
+      f[i] = z < 64 ? by : 0.f;
+      v[i] = z < 64 ? *reinterpret_cast<const f32x4*>(po + (size_t)z * kDim) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a += v[i] * f[i];
   }
   const float inv = 1.f / sum;
-  bf16* op = p.out + (size_t)row * kDim + 2 * lane;
-  op[0] = f2bf(a * inv);
-  op[1] = f2bf(b * inv);
+  bf16x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = f2bf((a[i] + __shfl_xor(a[i], 32)) * inv);
+  if (lane < 32) *reinterpret_cast<bf16x4*>(p.out + (size_t)row * kDim + 4 * lane) = out;
 }
 
 // one wave per group: leading table columns, whole pages of every live beam, that are the same in all of them
@@ -247,6 +366,24 @@ __global__ void __launch_bounds__(64) beam_shared_kernel(const int* tables, cons
   if (lane == 0) shared[g] = found;
 }
 
+template <int T>
+hipError_t launch_attention(dim3 grid, const BeamAttnParams& p, hipStream_t st) {
+  constexpr int NW = waves_of(T), join = NW * (32 * 64 + 32) * 4, lds = T > 1 && kRing * 2 * kHalf > join ? kRing * 2 * kHalf : join;
+  if (lds > 64 * 1024) {  // once per device
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == hipSuccess && !(set.load(std::memory_order_relaxed) & bit)) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&beam_attention_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e == hipSuccess) set.fetch_or(bit, std::memory_order_relaxed);
+    }
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(beam_attention_kernel<T>, grid, dim3(64 * NW), lds, st, p);
+  return hipGetLastError();
+}
+
 }  // namespace
 }  // namespace dsse
 
@@ -254,7 +391,7 @@ __global__ void __launch_bounds__(64) beam_shared_kernel(const int* tables, cons
 // stands for them.
 extern "C" void dsse_beam_plan(dsse::BeamAttnParams* p) {
   const int cols = p->width * p->group, groups = p->slots / p->width;
-  p->tiles = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+  p->tiles = cols <= 16 ? 1 : (cols <= 32 ? 2 : (cols <= 64 ? 4 : 8));
   p->col_blocks = (cols + 16 * p->tiles - 1) / (16 * p->tiles);
   auto cut = [&](int64_t items, int most) {
     const int64_t n = items >= 512 ? 1 : (512 + items - 1) / items;
@@ -271,11 +408,13 @@ extern "C" hipError_t dsse_beam_attention(const dsse::BeamAttnParams* p, hipStre
       p->ns + p->no > 64 || p->hkv > 65535)
     return hipErrorInvalidValue;
   const int groups = p->slots / p->width;
-  const dim3 grid(groups * p->col_blocks * p->ns + p->slots * p->no, p->hkv), block(64 * kBeamWaves);
-  if (p->tiles == 1) hipLaunchKernelGGL((beam_attention_kernel<1>), grid, block, 0, st, *p);
-  else if (p->tiles == 2) hipLaunchKernelGGL((beam_attention_kernel<2>), grid, block, 0, st, *p);
-  else if (p->tiles == 4) hipLaunchKernelGGL((beam_attention_kernel<4>), grid, block, 0, st, *p);
-  else return hipErrorInvalidValue;
+  const dim3 grid(groups * p->col_blocks * p->ns + p->slots * p->no, p->hkv);
+  hipError_t e = hipErrorInvalidValue;
+  if (p->tiles == 1) e = launch_attention<1>(grid, *p, st);
+  else if (p->tiles == 2) e = launch_attention<2>(grid, *p, st);
+  else if (p->tiles == 4) e = launch_attention<4>(grid, *p, st);
+  else if (p->tiles == 8) e = launch_attention<8>(grid, *p, st);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL(beam_join_kernel, dim3((p->slots * p->hq + 3) / 4), dim3(256), 0, st, *p);
   return hipGetLastError();
 }
