@@ -7,9 +7,15 @@
 //   work items  x < groups * col_blocks * ns: the shared keys of a group, a block of columns, one of ns parts
 //               else                        : a slot's own keys, one of no parts
 //
-// T = 1 (up to 16 columns): four waves take the pages in turn, straight to registers, and join their sums in LDS.
+// for every key/value head, heads first, parts last: workgroups go to the XCDs and CUs in turn, so the long walks have to be
+// neighbours, and so have the first parts of short walks, whose last ones are empty (16x4 beams of 512 + 100 tokens with 32 parts in
+// place of 4: 54 us with the part as the fastest index, 26 as it is; 2x16 of 31077 tokens 29.7, with the heads last 36).
+//
+// T = 1 (up to 16 columns): four waves take the pages in turn, straight to registers, and join their sums in LDS; a slot's own pages
+// go to two waves in the same way, several slots to a workgroup.
 // T = 2, 4, 8: a wave per column tile; the pages pass through LDS once for all waves, filled by LDS-DMA kRing - 1 pages ahead.  A
-// page costs 16 KB from memory and T tiles' products, so what bounds it is memory; the ring keeps it busy with one wave per SIMD.
+// page costs 16 KB from memory and T tiles' products, so what bounds it is memory.  A ring of 5 pages lets one workgroup on a CU
+// where one of 3 lets three: 2x16 beams of 31077 tokens 36 -> 28.6 us.
 //
 // Statistics and sums in fp32; scores in base 2 with the scale folded in; weights rounded to bf16 for the second product, as in
 // paged_attention.
@@ -24,7 +30,8 @@ namespace {
 constexpr int kPg = 32;
 constexpr int kDim = 128;
 constexpr int kHalf = kPg * kDim * 2;  // bytes of a page's keys, or of its values
-constexpr int kRing = 5;               // pages in LDS; two workgroups of a CU fill its 160 KB
+constexpr int kRing = 3;               // pages in LDS: three workgroups of a CU keep six pages on their way
+constexpr int kOwnWaves = 2;           // waves that split a slot's own pages
 constexpr float kLow = -1e30f;         // a finite start: fully masked columns stay finite and sum to zero
 
 constexpr int waves_of(int T) { return T == 1 ? 4 : T; }
@@ -104,14 +111,16 @@ DEV void blank_values(bf16x8 (&vf)[8], int left) {
 }
 
 // Keys of pages [pb, pe) up to `limit`, for 16 columns, pages in turn to NW waves
-template <int NW>
+template <int NW, bool ONCE>
 DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int limit, int row, Column& c) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
+  auto load = [](const bf16* at) { return ONCE ? ld_once<bf16x8>(at) : ld_global<bf16x8>(at); };
   bf16x8 qf[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) qf[k] = row >= 0 ? ld_bf16x8(p.q + (size_t)row * kDim + 32 * k + 8 * g) : zero_bf16x8();
   c.clear();
-  int id = entry(bt, min(pb + kw, pe - 1));
+  if (pb + kw >= pe) return;
+  int id = entry(bt, pb + kw);
   for (int pg = pb + kw; pg < pe; pg += NW) {
     const size_t at = ((size_t)page_of(p, id) * p.hkv + h) * kPg * kDim;
     id = entry(bt, min(pg + NW, pe - 1));  // the next one is on its way while this page is computed
@@ -119,11 +128,11 @@ DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int
     bf16x8 k0[4], k1[4], vf[8];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      k0[s] = ld_once<bf16x8>(kp + r * kDim + 32 * s + 8 * g);
-      k1[s] = ld_once<bf16x8>(kp + (16 + r) * kDim + 32 * s + 8 * g);
+      k0[s] = load(kp + r * kDim + 32 * s + 8 * g);
+      k1[s] = load(kp + (16 + r) * kDim + 32 * s + 8 * g);
     }
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) vf[dt] = ld_once<bf16x8>(vp + (16 * dt + r) * kPg + 8 * g);
+    for (int dt = 0; dt < 8; ++dt) vf[dt] = load(vp + (16 * dt + r) * kPg + 8 * g);
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -139,7 +148,7 @@ DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int
 }
 
 // The same for T column tiles, one per wave: whole pages [pb, pe) through LDS
-template <int T>
+template <int T, bool ONCE>
 DEV void walk_tiles(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int row, Column& c, char* smem) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // head dims of a k-step: 32 g + 8 s .. + 7 of both operands
@@ -170,7 +179,7 @@ DEV void walk_tiles(const BeamAttnParams& p, const int* bt, int h, int pb, int p
     char* to = smem + slot_in * 2 * kHalf + wave * IPW * 1024;
     slot_in = slot_in + 1 == kRing ? 0 : slot_in + 1;
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) lds_dma<kAuxNT>(src, to + i * 1024, from[i]);
+    for (int i = 0; i < IPW; ++i) lds_dma<ONCE ? kAuxNT : 0>(src, to + i * 1024, from[i]);
   };
   int kofs[4];
 #pragma unroll
@@ -216,11 +225,13 @@ DEV void leave(const BeamAttnParams& p, const Column& c, int row, int z) {
   if (g == 0) p.part_ml[(size_t)row * np + z] = make_float2(c.m, l);
 }
 
-// The same for waves that split the keys of one column tile: joined in LDS, wave kw the head dims 128 kw / NW ..
+// The same for groups of NW waves that split the keys of one column tile: joined in LDS, wave kw of a group the head dims
+// 128 kw / NW ..  Every wave of the workgroup comes here.
+constexpr int join_bytes(int waves) { return waves * (32 * 64 + 32) * 4; }
 template <int NW>
 DEV void leave_joined(const BeamAttnParams& p, const Column& c, int row, int z, char* smem) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = threadIdx.x >> 6, np = p.ns + p.no;
-  float* o = reinterpret_cast<float*>(smem);   // [NW][32][64]
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6, kw = wave % NW, np = p.ns + p.no;
+  float* o = reinterpret_cast<float*>(smem + wave / NW * join_bytes(NW));  // [NW][32][64]
   float* ms = o + NW * 32 * 64;                // [NW][16]
   float* ls = ms + NW * 16;
   const float own = rows4_sum(c.l);
@@ -260,17 +271,17 @@ DEV int2 part_of(int pages, int n, int z, int least) {
   return make_int2(pb, min(pages, pb + per));
 }
 
-template <int T>
+template <int T, bool ONCE>
 __global__ void __launch_bounds__(64 * waves_of(T), 2) beam_attention_kernel(BeamAttnParams p) {
   constexpr int NW = waves_of(T);
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15;
-  const int h = blockIdx.y, np = p.ns + p.no;
-  const int nshared = p.slots / p.width * p.col_blocks * p.ns;
+  const int h = blockIdx.x % p.hkv, x = blockIdx.x / p.hkv, np = p.ns + p.no;
+  const int groups = p.slots / p.width, nshared = groups * p.col_blocks * p.ns;
   int live;
   Column c;
-  if ((int)blockIdx.x < nshared) {
-    const int z = blockIdx.x % p.ns, cb = blockIdx.x / p.ns % p.col_blocks, gr = blockIdx.x / (p.ns * p.col_blocks);
+  if (x < nshared) {
+    const int cb = x % p.col_blocks, gr = x / p.col_blocks % groups, z = x / (p.col_blocks * groups);
     const int2 part = part_of(group_pages(p, gr, live), p.ns, z, 4);
     const int at = (cb * T + (T == 1 ? 0 : threadIdx.x >> 6)) * 16 + r, w = at / p.group, s = gr * p.width + w;
     const int row = w < p.width && p.ctx_len[s] > 0 ? s * p.hq + h * p.group + at % p.group : -1;
@@ -280,25 +291,25 @@ __global__ void __launch_bounds__(64 * waves_of(T), 2) beam_attention_kernel(Bea
     }
     const int* bt = p.block_tables + (size_t)live * p.max_blocks;
     if constexpr (T == 1) {
-      walk<NW>(p, bt, h, part.x, part.y, part.y * kPg, row, c);
+      walk<NW, ONCE>(p, bt, h, part.x, part.y, part.y * kPg, row, c);
       leave_joined<NW>(p, c, row, z, smem);
     } else {
-      walk_tiles<T>(p, bt, h, part.x, part.y, row, c, smem);
+      walk_tiles<T, ONCE>(p, bt, h, part.x, part.y, row, c, smem);
       leave(p, c, row, z);
     }
   } else {
-    const int x = blockIdx.x - nshared, z = x % p.no, s = x / p.no;
-    const int n = p.ctx_len[s];
-    if (n <= 0) return;
+    constexpr int kGroups = NW / kOwnWaves;
+    const int item = (x - nshared) * kGroups + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kOwnWaves;
+    const int s = item % p.slots, z = item / p.slots, n = z < p.no ? p.ctx_len[s] : 0;
+    const int row = n > 0 && r < p.group ? s * p.hq + h * p.group + r : -1;
     const int skip = group_pages(p, s / p.width, live);
-    const int2 part = part_of(min((n + kPg - 1) / kPg, p.max_blocks) - skip, p.no, z, NW);
-    const int row = r < p.group ? s * p.hq + h * p.group + r : -1;
-    if (part.x >= part.y) {
-      if (threadIdx.x < 16 && row >= 0) p.part_ml[(size_t)row * np + p.ns + z] = make_float2(kLow, 0.f);
+    const int2 part = part_of(n > 0 ? min((n + kPg - 1) / kPg, p.max_blocks) - skip : 0, p.no, z, 2 * kOwnWaves);
+    if (!__syncthreads_or(part.x < part.y)) {
+      if (lane < 16 && row >= 0) p.part_ml[(size_t)row * np + p.ns + z] = make_float2(kLow, 0.f);
       return;
     }
-    walk<NW>(p, p.block_tables + (size_t)s * p.max_blocks, h, skip + part.x, skip + part.y, n, row, c);
-    leave_joined<NW>(p, c, row, p.ns + z, smem);
+    walk<kOwnWaves, ONCE>(p, p.block_tables + (size_t)s * p.max_blocks, h, skip + part.x, skip + part.y, n, row, c);
+    leave_joined<kOwnWaves>(p, c, row, p.ns + z, smem);
   }
 }
 
@@ -366,21 +377,27 @@ __global__ void __launch_bounds__(64) beam_shared_kernel(const int* tables, cons
   if (lane == 0) shared[g] = found;
 }
 
-template <int T>
+// Pages of a layer that fill less than half of the 256 MB memory-side cache may still be there when they are read next; others only
+// wash it through, and non-temporal loads are the faster.  Measured, those against the default, three pools in turn: 64 MB each 26 / 24
+// us, 92 MB (16x4 beams of 612 tokens) 18.3 / 14.8, 95 MB 23.7 / 18.9, 134 MB (2x16 of 31077) 29.7 / 33.1, 300 MB 50 / 54, 371 MB (8x8
+// of 8300) 62 / 70.
+constexpr int64_t kStays = 112 << 20;
+
+template <int T, bool ONCE>
 hipError_t launch_attention(dim3 grid, const BeamAttnParams& p, hipStream_t st) {
-  constexpr int NW = waves_of(T), join = NW * (32 * 64 + 32) * 4, lds = T > 1 && kRing * 2 * kHalf > join ? kRing * 2 * kHalf : join;
+  constexpr int NW = waves_of(T), ring = T > 1 ? kRing * 2 * kHalf : 0, lds = ring > join_bytes(NW) ? ring : join_bytes(NW);
   if (lds > 64 * 1024) {  // once per device
     static std::atomic<uint64_t> set{0};
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (e == hipSuccess && !(set.load(std::memory_order_relaxed) & bit)) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&beam_attention_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&beam_attention_kernel<T, ONCE>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (e == hipSuccess) set.fetch_or(bit, std::memory_order_relaxed);
     }
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(beam_attention_kernel<T>, grid, dim3(64 * NW), lds, st, p);
+  hipLaunchKernelGGL((beam_attention_kernel<T, ONCE>), grid, dim3(64 * NW), lds, st, p);
   return hipGetLastError();
 }
 
@@ -388,18 +405,20 @@ hipError_t launch_attention(dim3 grid, const BeamAttnParams& p, hipStream_t st) 
 }  // namespace dsse
 
 // Column tiles of a workgroup and cuts of the walks, from what the host knows: the lengths are on the device, so the tables' width
-// stands for them.
+// stands for them.  Shared walks: a workgroup per CU where it holds four tiles or more (4x16 beams of 16 heads and 16077 tokens
+// 28.9 us with 16 parts, 35 with 32), two where it holds fewer.  Own walks: eight waves per CU.
 extern "C" void dsse_beam_plan(dsse::BeamAttnParams* p) {
+  using namespace dsse;
   const int cols = p->width * p->group, groups = p->slots / p->width;
   p->tiles = cols <= 16 ? 1 : (cols <= 32 ? 2 : (cols <= 64 ? 4 : 8));
   p->col_blocks = (cols + 16 * p->tiles - 1) / (16 * p->tiles);
-  auto cut = [&](int64_t items, int most) {
-    const int64_t n = items >= 512 ? 1 : (512 + items - 1) / items;
+  auto cut = [](int64_t want, int64_t items, int most) {
+    const int64_t n = (want + items - 1) / items;
     return (int)(n < most ? n : most);
   };
-  const int by4 = (p->max_blocks + 3) / 4;  // a page per wave
-  p->ns = cut((int64_t)groups * p->col_blocks * p->hkv, by4 < 32 ? by4 : 32);
-  p->no = cut((int64_t)p->slots * p->hkv, by4 < 8 ? by4 : 8);
+  const int by4 = (p->max_blocks + 3) / 4;
+  p->ns = cut(p->tiles >= 4 ? 256 : 512, (int64_t)groups * p->col_blocks * p->hkv, by4 < 48 ? by4 : 48);
+  p->no = cut(512, (int64_t)p->slots * p->hkv, by4 < 16 ? by4 : 16);
 }
 
 extern "C" hipError_t dsse_beam_attention(const dsse::BeamAttnParams* p, hipStream_t st) {
@@ -408,12 +427,14 @@ extern "C" hipError_t dsse_beam_attention(const dsse::BeamAttnParams* p, hipStre
       p->ns + p->no > 64 || p->hkv > 65535)
     return hipErrorInvalidValue;
   const int groups = p->slots / p->width;
-  const dim3 grid(groups * p->col_blocks * p->ns + p->slots * p->no, p->hkv);
+  const int per = waves_of(p->tiles) / kOwnWaves;  // own walks of a workgroup
+  const dim3 grid((groups * p->col_blocks * p->ns + (p->slots * p->no + per - 1) / per) * p->hkv);
+  const bool once = (int64_t)p->num_blocks * p->hkv * 2 * kHalf > kStays;
   hipError_t e = hipErrorInvalidValue;
-  if (p->tiles == 1) e = launch_attention<1>(grid, *p, st);
-  else if (p->tiles == 2) e = launch_attention<2>(grid, *p, st);
-  else if (p->tiles == 4) e = launch_attention<4>(grid, *p, st);
-  else if (p->tiles == 8) e = launch_attention<8>(grid, *p, st);
+  if (p->tiles == 1) e = once ? launch_attention<1, true>(grid, *p, st) : launch_attention<1, false>(grid, *p, st);
+  else if (p->tiles == 2) e = once ? launch_attention<2, true>(grid, *p, st) : launch_attention<2, false>(grid, *p, st);
+  else if (p->tiles == 4) e = once ? launch_attention<4, true>(grid, *p, st) : launch_attention<4, false>(grid, *p, st);
+  else if (p->tiles == 8) e = once ? launch_attention<8, true>(grid, *p, st) : launch_attention<8, false>(grid, *p, st);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(beam_join_kernel, dim3((p->slots * p->hq + 3) / 4), dim3(256), 0, st, *p);
   return hipGetLastError();
