@@ -11,7 +11,7 @@ constexpr int kBeamWidth = 32;  // beams of a group
 constexpr int kBeamKeep = 64;   // candidates of a group
 constexpr int kForkSlots = 2048;
 constexpr int kReorderLists = 96;  // tensors of one launch (24 bytes each of a kernel's arguments)
-constexpr int kCopyPools = 96;
+constexpr int kCopyPools = 64;     // (32 bytes each)
 
 struct BeamSelectParams {
   const void* logits;   // [rows, V] rows ld apart
@@ -49,16 +49,19 @@ struct PageForkParams {
   int* refs;           // [pages] holders of each page
   int* copies;         // [slots, 2] source, destination; -1 without a copy
   int* starved;        // [1] slots that found no free page
+  int* list;           // [1 + slots] how many slots copy, which
   int slots, max_blocks, pages;
 };
 
 struct PageCopyParams {
   const int* copies;  // [slots, 2]
-  int slots, pages, npools;
+  const int* list;    // [1 + slots]
+  int slots, npools, blocks;  // blocks: of a slot, over all pools
   struct Pool {
     char* base;
-    int64_t layer;  // bytes from a layer to the next
+    int64_t layer;      // bytes from a layer to the next
     int layers, bytes;  // bytes of a page
+    int per, first;     // workgroups of a layer's page, the pool's first one (set by the launcher)
   } pool[kCopyPools];
 };
 

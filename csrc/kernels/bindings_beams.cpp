@@ -42,6 +42,15 @@ int beams(int64_t slots, int64_t width) {
   TORCH_CHECK(slots % width == 0, "slots must be whole groups of `width` beams");
   return (int)(slots / width);
 }
+// whether the dimensions from `first` on are one contiguous run
+bool packed(const Tensor& t, int64_t first) {
+  int64_t run = 1;
+  for (int64_t d = t.dim() - 1; d >= first; --d) {
+    if (t.size(d) != 1 && t.stride(d) != run) return false;
+    run *= t.size(d);
+  }
+  return true;
+}
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 void beam_select(const Tensor& logits, const Tensor& scores, Tensor& out_scores, Tensor& out_rows, Tensor& out_tokens, int64_t eos_id,
@@ -166,7 +175,7 @@ void page_fork(Tensor& block_tables, Tensor& held, Tensor& lens, const Tensor& p
     on(t, block_tables, "pool", false);
     TORCH_CHECK(t.dim() >= 3 && t.size(1) == pages, "a pool must be [layers, pages, ..]");
     if (t.numel() == 0) continue;
-    TORCH_CHECK(t.select(0, 0).is_contiguous() && (t.size(0) == 1 || t.stride(0) >= t.stride(1) * pages), "a pool's pages must be contiguous");
+    TORCH_CHECK(packed(t, 1) && (t.size(0) == 1 || t.stride(0) >= t.numel() / t.size(0)), "a pool's pages must be contiguous");
     const int64_t bytes = t.numel() / t.size(0) / pages * t.element_size();
     TORCH_CHECK(bytes % 16 == 0 && bytes < INT_MAX && aligned16(t.data_ptr()) && (t.size(0) == 1 || t.stride(0) * t.element_size() % 16 == 0),
                 "a pool's pages must start and end at 16 bytes");
@@ -174,16 +183,17 @@ void page_fork(Tensor& block_tables, Tensor& held, Tensor& lens, const Tensor& p
   if (S == 0) return;
   const c10::DeviceGuard guard(block_tables.device());
   const hipStream_t st = stream_of(block_tables);
+  Tensor list = at::empty({S + 1}, block_tables.options());
   dsse::PageForkParams p{block_tables.data_ptr<int>(), held.data_ptr<int>(), lens.data_ptr<int>(), parents.data_ptr<int>(), refs.data_ptr<int>(),
-                         copies.data_ptr<int>(), starved.data_ptr<int>(), (int)S, (int)block_tables.size(1), (int)pages};
+                         copies.data_ptr<int>(), starved.data_ptr<int>(), list.data_ptr<int>(), (int)S, (int)block_tables.size(1), (int)pages};
   DSSE_CHECK_HIP(dsse_page_fork(&p, st));
   dsse::PageCopyParams c{};
-  c.copies = p.copies, c.slots = p.slots, c.pages = p.pages;
+  c.copies = p.copies, c.list = p.list, c.slots = p.slots;
   for (size_t i = 0; i < pools.size(); ++i) {
     const Tensor& t = pools[i];
     if (t.numel() > 0)
       c.pool[c.npools++] = {reinterpret_cast<char*>(t.data_ptr()), t.size(0) == 1 ? 0 : t.stride(0) * (int64_t)t.element_size(), (int)t.size(0),
-                            (int)(t.numel() / t.size(0) / pages * t.element_size())};
+                            (int)(t.numel() / t.size(0) / pages * t.element_size()), 0, 0};
     if (c.npools == dsse::kCopyPools || (i + 1 == pools.size() && c.npools > 0)) {
       DSSE_CHECK_HIP(dsse_page_copy(&c, st));
       c.npools = 0;
@@ -201,7 +211,7 @@ void state_reorder(at::TensorList states, const Tensor& parents, int64_t width) 
     TORCH_CHECK(t.dim() >= 1 && t.size(0) == S, "a state must be [slots, ..]");
     if (t.numel() == 0) continue;
     const int64_t row = t.numel() / S;
-    TORCH_CHECK(t.select(0, 0).is_contiguous() && (S == 1 || t.stride(0) >= row), "a slot's state must be contiguous");
+    TORCH_CHECK(packed(t, 1) && (S == 1 || t.stride(0) >= row), "a slot's state must be contiguous");
     TORCH_CHECK(row * t.element_size() % 2 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 2 == 0 &&
                     (S == 1 || t.stride(0) * t.element_size() % 2 == 0) && row * t.element_size() < INT_MAX - (1 << 16),
                 "a slot's state must have an even number of bytes, under 2 GiB");

@@ -1,10 +1,11 @@
 // Forks of paged sequences: slot s goes on with the pages that slot parents[s] holds.  Full pages are shared (refs counts a page's
 // holders, 0 = free); the page that a slot's next token goes to becomes its own.  Three launches:
 //
-//   tables  every workgroup takes a strip of 16 columns of the tables, reads what the slots give up and take over, counts holders
+//   tables  every workgroup takes a strip of 4 columns of the tables, reads what the slots give up and take over, counts holders
 //           down and up where the two differ (integer atomics: the order does not matter), and writes the strip after its last read.
 //   pages   one workgroup: who needs a page of its own, the lowest free ones in slot order, counts, lengths, the list of copies.
-//   copies  the listed pages of every pool and layer, 16 bytes a lane.
+//   copies  the listed pages of every pool and layer, 64 bytes a lane in flight; workgroups walk the list, whose length only the
+//           device knows.
 //
 // Beams of a request have the same pages but for the last few, so the first launch is two reads of the tables and few atomics; the
 // copies are what costs, two passes over each page.
@@ -12,9 +13,10 @@
 
 namespace dsse {
 
-constexpr int kStrip = 16;          // columns of a workgroup of the first launch
+constexpr int kStrip = 4;           // columns of a workgroup of the first launch
 constexpr int kForkThreads = 1024;
 constexpr int kCopyThreads = 256;
+constexpr int kCopyUnits = 4;       // 16-byte units of a lane
 
 DEV bool goes_on(int parent, int slots) { return (unsigned)parent < (unsigned)slots; }
 
@@ -24,26 +26,25 @@ __global__ void __launch_bounds__(kForkThreads) fork_tables_kernel(PageForkParam
   const int j = blockIdx.x * kStrip + threadIdx.x % kStrip;
   const int s0 = threadIdx.x / kStrip;
   constexpr int kStep = kForkThreads / kStrip;  // slots of a pass
-  int next[N];
+  int next[N], old[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int s = s0 + n * kStep;
-    next[n] = -1;
+    next[n] = old[n] = -1;
     if (s >= p.slots || j >= p.max_blocks) continue;
     const int q = p.parents[s];
     if (q == s) continue;
-    const bool on = goes_on(q, p.slots);
-    const int old = j < p.held[s] ? p.tables[(size_t)s * p.max_blocks + j] : -1;
-    if (on && j < p.held[q]) next[n] = p.tables[(size_t)q * p.max_blocks + j];
-    if (old != next[n]) {
-      if ((unsigned)old < (unsigned)p.pages) atomicSub(&p.refs[old], 1);
-      if ((unsigned)next[n] < (unsigned)p.pages) atomicAdd(&p.refs[next[n]], 1);
-    }
+    if (j < p.held[s]) old[n] = p.tables[(size_t)s * p.max_blocks + j];
+    if (goes_on(q, p.slots) && j < p.held[q]) next[n] = p.tables[(size_t)q * p.max_blocks + j];
   }
   __syncthreads();  // the strip is read: it may change
 #pragma unroll
-  for (int n = 0; n < N; ++n)
+  for (int n = 0; n < N; ++n) {
+    if (old[n] == next[n]) continue;  // most of the pages that beams of a request hold
+    if ((unsigned)old[n] < (unsigned)p.pages) atomicSub(&p.refs[old[n]], 1);
+    if ((unsigned)next[n] < (unsigned)p.pages) atomicAdd(&p.refs[next[n]], 1);
     if (next[n] >= 0) p.tables[(size_t)(s0 + n * kStep) * p.max_blocks + j] = next[n];
+  }
 }
 
 // exclusive prefix sum over the workgroup; total: the sum
@@ -71,6 +72,16 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
   __shared__ int follow[kForkSlots], last[kForkSlots], fresh[kForkSlots], scan[kForkThreads / 64];
   constexpr int kPer = kForkSlots / kForkThreads;  // neighbouring slots of a thread
   const int s0 = threadIdx.x * kPer;
+  // counts of four neighbouring pages, on their way while the slots are looked at
+  int count[4];
+  auto look = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = base + threadIdx.x * 4 + k;
+      count[k] = i < p.pages ? p.refs[i] : 1;
+    }
+  };
+  look(0);
   for (int i = threadIdx.x; i < kForkSlots; i += kForkThreads) follow[i] = 0, last[i] = -1;
   __syncthreads();
   int parent[kPer], len[kPer], held[kPer];
@@ -108,10 +119,10 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
     int at[4], n = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = base + threadIdx.x * 4 + k;
-      at[k] = i < p.pages && p.refs[i] == 0 ? 1 : 0;
+      at[k] = count[k] == 0 ? 1 : 0;
       n += at[k];
     }
+    look(base + kForkThreads * 4);
     int all, to = block_scan(n, scan, all) + found;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -123,6 +134,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
   }
   __syncthreads();  // free pages are chosen: the counts may change
   const int had = found < wanted ? found : wanted;
+  int copied = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int s = s0 + i;
@@ -145,22 +157,36 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
     p.lens[s] = len[i];
     p.copies[2 * s] = src;
     p.copies[2 * s + 1] = dst;
+    if (src >= 0) copied |= 1 << i;
   }
-  if (threadIdx.x == 0) p.starved[0] = wanted - had;
+  int copies, at = block_scan(__popc(copied), scan, copies);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (copied >> i & 1) p.list[1 + at++] = s0 + i;
+  if (threadIdx.x == 0) {
+    p.starved[0] = wanted - had;
+    p.list[0] = copies;
+  }
 }
 
-// grid (pieces of a page, slots): the workgroups of a slot walk the layers of all pools
+// Work item: 16 KB of a page of a pool's layer, for one of the listed slots
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(PageCopyParams p) {
-  const int src = p.copies[2 * blockIdx.y], dst = p.copies[2 * blockIdx.y + 1];
-  if ((unsigned)src >= (unsigned)p.pages || (unsigned)dst >= (unsigned)p.pages) return;
-  for (int i = 0; i < p.npools; ++i) {
+  const int total = p.list[0] * p.blocks;
+  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    const int slot = p.list[1 + w / p.blocks], b = w % p.blocks;
+    const int src = p.copies[2 * slot], dst = p.copies[2 * slot + 1];
+    int i = 0;
+    while (i + 1 < p.npools && b >= p.pool[i + 1].first) ++i;
     const auto o = p.pool[i];
-    const int units = o.bytes / 16;
-    for (int64_t u = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; u < (int64_t)units * o.layers; u += (int64_t)gridDim.x * kCopyThreads) {
-      const int l = (int)(u / units), e = (int)(u % units);
-      char* base = o.base + l * o.layer + (int64_t)e * 16;
-      *reinterpret_cast<u32x4*>(base + (int64_t)dst * o.bytes) = *reinterpret_cast<const u32x4*>(base + (int64_t)src * o.bytes);
-    }
+    const int layer = (b - o.first) / o.per, e0 = (b - o.first) % o.per * kCopyThreads * kCopyUnits * 16 + threadIdx.x * 16;
+    const char* from = o.base + layer * o.layer + (int64_t)src * o.bytes;
+    char* to = o.base + layer * o.layer + (int64_t)dst * o.bytes;
+    u32x4 v[kCopyUnits];
+#pragma unroll
+    for (int u = 0; u < kCopyUnits; ++u) v[u] = ld_global<u32x4>(from + min(e0 + u * kCopyThreads * 16, o.bytes - 16));
+#pragma unroll
+    for (int u = 0; u < kCopyUnits; ++u)
+      if (e0 + u * kCopyThreads * 16 < o.bytes) *reinterpret_cast<u32x4*>(to + e0 + u * kCopyThreads * 16) = v[u];
   }
 }
 
@@ -171,17 +197,26 @@ extern "C" hipError_t dsse_page_fork(const dsse::PageForkParams* p, hipStream_t 
   if (p->slots < 1 || p->slots > kForkSlots || p->max_blocks < 1 || p->pages < 1) return hipErrorInvalidValue;
   const dim3 grid((p->max_blocks + kStrip - 1) / kStrip), block(kForkThreads);
   constexpr int kStep = kForkThreads / kStrip;
-  const int per = (p->slots + kStep - 1) / kStep;
-  if (per <= 1) hipLaunchKernelGGL((fork_tables_kernel<1>), grid, block, 0, st, *p);
-  else if (per <= 8) hipLaunchKernelGGL((fork_tables_kernel<8>), grid, block, 0, st, *p);
+  if (p->slots <= kStep) hipLaunchKernelGGL((fork_tables_kernel<1>), grid, block, 0, st, *p);
   else hipLaunchKernelGGL((fork_tables_kernel<kForkSlots / kStep>), grid, block, 0, st, *p);
   hipLaunchKernelGGL(fork_pages_kernel, dim3(1), block, 0, st, *p);
   return hipGetLastError();
 }
 
-extern "C" hipError_t dsse_page_copy(const dsse::PageCopyParams* p, hipStream_t st) {
+extern "C" hipError_t dsse_page_copy(const dsse::PageCopyParams* in, hipStream_t st) {
   using namespace dsse;
-  if (p->slots < 1 || p->slots > 65535 || p->npools < 1 || p->npools > kCopyPools) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(page_copy_kernel, dim3(64, p->slots), dim3(kCopyThreads), 0, st, *p);
+  if (in->slots < 1 || in->slots > kForkSlots || in->npools < 1 || in->npools > kCopyPools) return hipErrorInvalidValue;
+  PageCopyParams p = *in;
+  constexpr int kBlock = kCopyThreads * kCopyUnits * 16;
+  int64_t blocks = 0;
+  for (int i = 0; i < p.npools; ++i) {
+    p.pool[i].per = (p.pool[i].bytes + kBlock - 1) / kBlock;
+    p.pool[i].first = (int)blocks;
+    blocks += (int64_t)p.pool[i].per * p.pool[i].layers;
+    if (blocks * p.slots > 0x7fffffff) return hipErrorInvalidValue;
+  }
+  p.blocks = (int)blocks;
+  const int64_t most = blocks * p.slots;  // all slots copy
+  hipLaunchKernelGGL(page_copy_kernel, dim3((unsigned)(most < 2048 ? most : 2048)), dim3(kCopyThreads), 0, st, p);
   return hipGetLastError();
 }
