@@ -3,9 +3,9 @@
 // by (score descending, row ascending, token ascending), in two launches.
 //
 // rows   one workgroup per (row, chunk of the vocabulary).  A chunk stays in registers: its maximum, the sum of exponentials about
-//        it, then its K best logits (within a row the order of the logits is the order of the scores).  The K-th best of 64
-//        buckets' maxima (bucket = lane) bounds the chunk's K-th best from below; what reaches it (1.2 K values where they fall at
-//        random) is gathered in LDS, and a value's place is the number of gathered ones before it.  No sort, no second read.
+//        it, then its K best logits (within a row the order of the logits is the order of the scores).  The K-th best of some
+//        buckets' maxima bounds the chunk's K-th best from below; what reaches it (1.2 K values where they fall at random) is gathered
+//        in LDS, and a value's place is the number of gathered ones before it.  No sort, no second read.
 // merge  one workgroup per group: the chunks' sums joined into each row's log-sum, the same selection over the rows' candidates.
 //
 // Two candidates of different rows may be nearer to each other than 32 bits of a score of tens tell, so scores are compared in 64
@@ -17,8 +17,8 @@ namespace {
 
 constexpr int kSelThreads = 256;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kGather = 512;  // candidates that LDS holds; a chunk or group with more that reach the bound (many equal logits, the best
-                              // ones all in a few lanes) is walked K times instead
+constexpr int kGather = 1024;  // candidates that LDS holds; a chunk or group with more that reach the bound (many equal logits, the best
+                               // ones all in a few threads) is walked K times instead
 
 // e^(x - m) for x <= m, by 2^y with y = (x - m) log2(e) in two parts
 DEV float exp_below(float x, float m) {
@@ -64,16 +64,17 @@ DEV V lane_value(V v, int lane) {  // a wave-uniform lane's value, without LDS
   return v;
 }
 
-// The K-th largest of 64 buckets' maxima, the same for every thread; mine: this thread's maximum, bucket = lane
+// The K-th largest of 64 buckets' maxima, the same for every thread; mine: this thread's maximum, bucket = lane.  Of the chunk's values
+// some 64 (H(64) - H(64 - K)) reach it: 1.1 K of them for K = 8, 1.4 K for 32, but 4.7 K for 64.
 template <typename V>
-DEV V bound_of(V mine, int K, V (*all)[64], int* rank) {
+DEV V bound_of_lanes(V mine, int K, V* all, int* rank) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  all[wave][lane] = mine;
+  all[threadIdx.x] = mine;
   if (wave == 0) rank[lane] = 0;
   __syncthreads();
-  V v = all[0][lane];
+  V v = all[lane];
 #pragma unroll
-  for (int w = 1; w < kSelWaves; ++w) v = all[w][lane] > v ? all[w][lane] : v;
+  for (int w = 1; w < kSelWaves; ++w) v = all[w * 64 + lane] > v ? all[w * 64 + lane] : v;
   int n = 0;  // buckets before this one, a quarter of them per wave; of equal ones the lower lane is before
 #pragma unroll
   for (int i = 0; i < 64 / kSelWaves; ++i) {
@@ -86,6 +87,23 @@ DEV V bound_of(V mine, int K, V (*all)[64], int* rank) {
   const unsigned long long who = __ballot(rank[lane] == K - 1);
   return lane_value(v, __ffsll(who) - 1);
 }
+// The same with a bucket per thread: nearer for many candidates, and for lists that are in order
+template <typename V>
+DEV V bound_of_threads(V mine, int K, V* all, int* rank) {
+  all[threadIdx.x] = mine;
+  if (threadIdx.x == 0) rank[0] = -1;
+  __syncthreads();
+  int n = 0;
+#pragma unroll 8
+  for (int i = 0; i < kSelThreads; ++i) n += all[i] > mine ? 1 : 0;
+  if (n < K) atomicMax(&rank[0], n);  // of the buckets with fewer than K above them, the lowest: equal ones have the same number
+  __syncthreads();
+  const bool is = n == rank[0];
+  __syncthreads();
+  if (is) all[0] = mine;
+  __syncthreads();
+  return all[0];
+}
 
 // Q: 16-byte pieces of a thread.  A row is whole pieces at 16-byte addresses and the few elements before and behind them, which go
 // to the first threads of its first workgroup, one each.
@@ -93,7 +111,7 @@ template <typename T, int Q>
 __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectParams p) {
   constexpr int N = Piece<T>::N;
   __shared__ float s_max[kSelWaves], s_sum[kSelWaves];
-  __shared__ float bucket[kSelWaves][64];
+  __shared__ float bucket[kSelThreads];
   __shared__ int rank[64], count;
   __shared__ uint64_t got[kGather];
   const int row = blockIdx.y, c = blockIdx.x;
@@ -157,7 +175,7 @@ __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectPar
   const float top = wave_max(ref);
   sum = wave_sum(sum * exp_below(ref, top));
   if (lane == 0) s_max[wave] = top, s_sum[wave] = sum;
-  const float bound = bound_of(m, p.K, bucket, rank);
+  const float bound = p.K <= 32 ? bound_of_lanes(m, p.K, bucket, rank) : bound_of_threads(m, p.K, bucket, rank);
   if (threadIdx.x == 0) {
     float all = s_max[0], s = 0.f;
 #pragma unroll
@@ -229,25 +247,39 @@ struct Pick {
   int id;  // beam of the group * V + token
 };
 DEV bool before(const Pick& a, const Pick& b) { return a.s > b.s || (a.s == b.s && a.id < b.id); }
+// n / d for whole numbers below 2^21, inv = 1 / d in 32 bits: half of one away from the next, where the product is off by 2^-22
+DEV int quotient(int n, float inv) { return (int)(((float)n + 0.5f) * inv); }
 
 __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParams p) {
-  constexpr int kHeld = 4;                               // candidates of a thread that its registers hold
-  __shared__ double base[kBeamWidth];                    // scores[row] - log(sum about `top`); NaN: the row offers nothing
+  constexpr int kHeld = 8;             // candidates of a thread that its registers hold
+  __shared__ double base[kBeamWidth];  // scores[row] - log(sum about `top`); NaN: the row offers nothing
   __shared__ float top[kBeamWidth];
-  __shared__ double bucket[kSelWaves][64];
-  __shared__ Pick gathered[2][kGather];
-  __shared__ int rank[64], count[2];
+  __shared__ double bucket[kSelThreads];
+  __shared__ Pick got[kGather];
+  __shared__ int rank[64], count, open[kHeld * kSelThreads], nopen;
   const int g = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x == 0) count[0] = count[1] = 0;
+  if (threadIdx.x == 0) count = nopen = 0;
   // The chunks' lists are in order: their first `deep` places are looked at, the others only where the last of those reaches the
-  // bound.  Candidate e: place e / lists of list e % lists -- neighbouring threads look at different lists.
+  // bound.  Neighbouring threads look at a list's places, each list from another one on: a row far ahead has its best in few lists, and
+  // they have to fall into different buckets.
   const int lists = p.width * p.chunks, deep = min(p.K, max(1, kHeld * kSelThreads / lists)), total = lists * deep;
+  const float by_deep = 1.f / (float)deep, by_chunks = 1.f / (float)p.chunks;
   const float2* cand = p.cand + (size_t)g * lists * p.K;
-  auto load = [&](int e) { return cand[(size_t)(e % lists) * p.K + e / lists]; };
+  auto spot = [&](int e, int& list) {  // candidate e's list and place
+    list = quotient(e, by_deep);
+    const int at = e - list * deep + 5 * list;
+    return at - quotient(at, by_deep) * deep;
+  };
+  auto load = [&](int e) {
+    int list;
+    const int at = spot(e, list);
+    return cand[(size_t)list * p.K + at];
+  };
   float2 held[kHeld];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) held[i] = load(min((int)threadIdx.x + i * kSelThreads, total - 1));
+  for (int i = 0; i < kHeld; ++i)
+    if (i == 0 || i * kSelThreads < total) held[i] = load(min((int)threadIdx.x + i * kSelThreads, total - 1));
   for (int w = threadIdx.x >> 4; w < p.width; w += kSelThreads / 16) {  // 16 lanes per row
     const float2* st = p.stat + (size_t)(g * p.width + w) * p.chunks;
     const int l = threadIdx.x & 15;
@@ -270,7 +302,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
   }
   __syncthreads();
   auto pick_of = [&](int list, float2 c) {
-    const int w = list / p.chunks;
+    const int w = quotient(list, by_chunks);
     const double b = base[w];
     Pick r{-INFINITY, 0x7fffffff};
     if (c.x > -INFINITY && b == b) r = Pick{b + ((double)c.x - (double)top[w]), w * p.V + __float_as_int(c.y)};
@@ -278,45 +310,51 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
   };
   // the looked-at candidates of this thread, those in registers first
   auto each = [&](auto f) {
+    int list;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int e = threadIdx.x + i * kSelThreads;
-      if (e < total) f(pick_of(e % lists, held[i]), e);
+      if (e >= total) return;
+      const int at = spot(e, list);
+      f(pick_of(list, held[i]), list, at);
     }
-    for (int e = threadIdx.x + kHeld * kSelThreads; e < total; e += kSelThreads) f(pick_of(e % lists, load(e)), e);
+    for (int e = threadIdx.x + kHeld * kSelThreads; e < total; e += kSelThreads) {
+      const int at = spot(e, list);
+      f(pick_of(list, load(e)), list, at);
+    }
   };
   double best = -INFINITY;
-  each([&](const Pick& c, int) { best = c.s > best ? c.s : best; });
-  const double bound = bound_of(best, p.K, bucket, rank);
+  each([&](const Pick& c, int, int) { best = c.s > best ? c.s : best; });
+  const double bound = p.K <= 32 ? bound_of_lanes(best, p.K, bucket, rank) : bound_of_threads(best, p.K, bucket, rank);
   auto gather = [&](const Pick& c) {
     const bool in = c.s >= bound && c.s > -INFINITY;
     if (in) {
-      const int at = atomicAdd(&count[0], 1);
-      if (at < kGather) gathered[0][at] = c;
+      const int at = atomicAdd(&count, 1);
+      if (at < kGather) got[at] = c;
     }
     return in;
   };
   if (best >= bound)
-    each([&](const Pick& c, int e) {
-      if (gather(c) && e / lists == deep - 1)
-        for (int at = deep; at < p.K && gather(pick_of(e % lists, cand[(size_t)(e % lists) * p.K + at])); ++at) {
-        }
+    each([&](const Pick& c, int list, int at) {
+      if (gather(c) && at == deep - 1 && deep < p.K) {
+        const int o = atomicAdd(&nopen, 1);
+        if (o < kHeld * kSelThreads) open[o] = list;
+        else count = kGather + 1;  // (more lists than threads' registers: all of them by place)
+      }
     });
   __syncthreads();
-  int n = count[0];
-  Pick* got = gathered[0];
-  if (n > 2 * p.K && n <= kGather) {
-    // A row far ahead has its best in few lists, and the lists' maxima say little: the same bound once more among the gathered
-    // ones, which lie in no order.
-    best = -INFINITY;
-    for (int a = threadIdx.x; a < n; a += kSelThreads) best = got[a].s > best ? got[a].s : best;
-    const double nearer = bound_of(best, p.K, bucket, rank);
-    for (int a = threadIdx.x; a < n; a += kSelThreads)
-      if (got[a].s >= nearer) gathered[1][atomicAdd(&count[1], 1)] = got[a];
+  const int opened = count <= kGather ? nopen : 0;
+  __syncthreads();  // every thread has read the counts: they may change
+  if (opened > 0) {  // the other places of the lists that go on, all at once
+    const int left = p.K - deep;
+    const float by_left = 1.f / (float)left;
+    for (int e = threadIdx.x; e < opened * left; e += kSelThreads) {
+      const int o = quotient(e, by_left), list = open[o];
+      gather(pick_of(list, cand[(size_t)list * p.K + deep + e - o * left]));
+    }
     __syncthreads();
-    n = count[1];
-    got = gathered[1];
   }
+  const int n = count;
   auto put = [&](int at, const Pick& c) {
     p.out_scores[(size_t)g * p.K + at] = (float)c.s;
     p.out_rows[(size_t)g * p.K + at] = g * p.width + c.id / p.V;
@@ -373,14 +411,14 @@ hipError_t launch_rows(const BeamSelectParams& p, hipStream_t st) {
 }  // namespace
 }  // namespace dsse
 
-// Pieces of a thread: as many as its registers hold, fewer while that leaves CUs empty
+// Pieces of a thread: as many as a row has and its registers hold, fewer while that leaves CUs empty
 extern "C" void dsse_beam_plan_rows(dsse::BeamSelectParams* p) {
-  const int n = p->f32 ? 4 : 8, row = (p->V + n - 1) / n;
-  for (p->pieces = 8;; p->pieces /= 2) {
-    const int chunk = p->pieces * dsse::kSelThreads;
-    p->chunks = (row + chunk - 1) / chunk;
-    if (p->pieces == 1 || (int64_t)p->rows * p->chunks >= 512) return;
-  }
+  const int n = p->f32 ? 4 : 8, row = (p->V + n - 1) / n, threads = dsse::kSelThreads;
+  p->pieces = 1;
+  while (p->pieces < 8 && p->pieces * threads < row) p->pieces *= 2;
+  auto chunks = [&] { return (row + p->pieces * threads - 1) / (p->pieces * threads); };
+  while (p->pieces > 1 && (int64_t)p->rows * chunks() < 512) p->pieces /= 2;
+  p->chunks = chunks();
 }
 
 extern "C" hipError_t dsse_beam_select(const dsse::BeamSelectParams* p, hipStream_t st) {

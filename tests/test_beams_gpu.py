@@ -100,6 +100,17 @@ def test_select_equal_logits(gpu):
         _same_choice(want, got)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("groups,width,V,K", [(1, 4, 50001, 64), (64, 8, 2100, 3)])
+def test_select_more_than_gathered(gpu, dtype, groups, width, V, K):
+    """Rows of equal logits, more of them than LDS holds candidates: in a workgroup of the rows, or over a row's workgroups."""
+    logits = torch.full((groups * width, V), -0.25, device=gpu, dtype=dtype)
+    scores = -torch.arange(groups * width, dtype=torch.float32).view(groups, width)
+    want, got = _select(gpu, logits, scores, K, 1)
+    assert got[1].tolist() == [[g * width] * K for g in range(groups)] and got[2][0].tolist() == [0] + list(range(2, K + 1))
+    _same_choice(want, got)
+
+
 def test_select_what_is_not_finite(gpu):
     gen = torch.Generator().manual_seed(3)
     logits = _logits(gen, 12, 3000, torch.float32)
