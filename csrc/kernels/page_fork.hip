@@ -1,5 +1,6 @@
 // Forks of paged sequences: slot s goes on with the pages that slot parents[s] holds.  Full pages are shared (refs counts a page's
-// holders, 0 = free); the page that a slot's next token goes to becomes its own.  Three launches:
+// holders, 0 = free); the page that a slot's next token goes to becomes its own.  Three launches, or two where the tables are
+// small enough for the workgroup of the second:
 //
 //   tables  every workgroup takes a strip of 4 columns of the tables, reads what the slots give up and take over, counts holders
 //           down and up where the two differ (integer atomics: the order does not matter), and writes the strip after its last read.
@@ -18,33 +19,47 @@ constexpr int kForkThreads = 1024;
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnits = 4;       // 16-byte units of a lane
 
-DEV bool goes_on(int parent, int slots) { return (unsigned)parent < (unsigned)slots; }
+constexpr int kSmall = 2;           // table entries of a thread of the second launch where it does without the first
 
-// N: table entries of a thread
-template <int N>
-__global__ void __launch_bounds__(kForkThreads) fork_tables_kernel(PageForkParams p) {
-  const int j = blockIdx.x * kStrip + threadIdx.x % kStrip;
-  const int s0 = threadIdx.x / kStrip;
-  constexpr int kStep = kForkThreads / kStrip;  // slots of a pass
+DEV bool goes_on(int parent, int slots) { return (unsigned)parent < (unsigned)slots; }
+// Counts are read past L1, which does not see the atomics of the same launch
+DEV int holders(const PageForkParams& p, int page) {
+  return __hip_atomic_load(&p.refs[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A workgroup's part of the tables, N entries of a thread; place(n, s, j): whether entry n is one, and which.  No entry outside of the
+// part is read or written: all columns of a slot are moved by themselves.
+template <int N, typename P>
+DEV void move_entries(const PageForkParams& p, P place) {
   int next[N], old[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    const int s = s0 + n * kStep;
+    int s, j;
     next[n] = old[n] = -1;
-    if (s >= p.slots || j >= p.max_blocks) continue;
+    if (!place(n, s, j)) continue;
     const int q = p.parents[s];
     if (q == s) continue;
     if (j < p.held[s]) old[n] = p.tables[(size_t)s * p.max_blocks + j];
     if (goes_on(q, p.slots) && j < p.held[q]) next[n] = p.tables[(size_t)q * p.max_blocks + j];
   }
-  __syncthreads();  // the strip is read: it may change
+  __syncthreads();  // the part is read: it may change
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    if (old[n] == next[n]) continue;  // most of the pages that beams of a request hold
+    int s, j;
+    if (!place(n, s, j) || old[n] == next[n]) continue;  // most of the pages that beams of a request hold
     if ((unsigned)old[n] < (unsigned)p.pages) atomicSub(&p.refs[old[n]], 1);
     if ((unsigned)next[n] < (unsigned)p.pages) atomicAdd(&p.refs[next[n]], 1);
-    if (next[n] >= 0) p.tables[(size_t)(s0 + n * kStep) * p.max_blocks + j] = next[n];
+    if (next[n] >= 0) p.tables[(size_t)s * p.max_blocks + j] = next[n];
   }
+}
+
+template <int N>
+__global__ void __launch_bounds__(kForkThreads) fork_tables_kernel(PageForkParams p) {
+  move_entries<N>(p, [&](int n, int& s, int& j) {
+    s = threadIdx.x / kStrip + n * (kForkThreads / kStrip);
+    j = blockIdx.x * kStrip + threadIdx.x % kStrip;
+    return s < p.slots && j < p.max_blocks;
+  });
 }
 
 // exclusive prefix sum over the workgroup; total: the sum
@@ -68,17 +83,27 @@ DEV int block_scan(int v, int* sh, int& total) {
   return before + x - v;
 }
 
+template <bool TABLES>
 __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams p) {
   __shared__ int follow[kForkSlots], last[kForkSlots], fresh[kForkSlots], scan[kForkThreads / 64];
   constexpr int kPer = kForkSlots / kForkThreads;  // neighbouring slots of a thread
   const int s0 = threadIdx.x * kPer;
+  if constexpr (TABLES) {
+    move_entries<kSmall>(p, [&](int n, int& s, int& j) {
+      const int e = n * kForkThreads + threadIdx.x;
+      s = e / p.max_blocks, j = e % p.max_blocks;
+      return s < p.slots;
+    });
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's counts have reached L2, where holders() reads
+    __syncthreads();
+  }
   // counts of four neighbouring pages, on their way while the slots are looked at
   int count[4];
   auto look = [&](int base) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = base + threadIdx.x * 4 + k;
-      count[k] = i < p.pages ? p.refs[i] : 1;
+      count[k] = i < p.pages ? holders(p, i) : 1;
     }
   };
   look(0);
@@ -106,7 +131,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
     if (j < held[i]) {
       page[i] = p.tables[(size_t)s * p.max_blocks + j];
       if ((unsigned)page[i] >= (unsigned)p.pages) { page[i] = -1; continue; }
-      if (last[q] == s && p.refs[page[i]] == follow[q]) continue;  // its followers alone hold it: the last one keeps it
+      if (last[q] == s && holders(p, page[i]) == follow[q]) continue;  // its followers alone hold it: the last one keeps it
     }
     mask |= 1 << i;
     ++need;
@@ -195,11 +220,17 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(PageCopyParams 
 extern "C" hipError_t dsse_page_fork(const dsse::PageForkParams* p, hipStream_t st) {
   using namespace dsse;
   if (p->slots < 1 || p->slots > kForkSlots || p->max_blocks < 1 || p->pages < 1) return hipErrorInvalidValue;
-  const dim3 grid((p->max_blocks + kStrip - 1) / kStrip), block(kForkThreads);
+  const dim3 block(kForkThreads);
+  // One launch of both against two, us without the gap between: 104 entries 6.3 / 8.0, 1536 9.8 / 10.8, 3264 and 7680 11.5 / 8.5 and 19.8 / 17
+  if ((int64_t)p->slots * p->max_blocks <= kSmall * kForkThreads) {
+    hipLaunchKernelGGL(fork_pages_kernel<true>, dim3(1), block, 0, st, *p);
+    return hipGetLastError();
+  }
+  const dim3 grid((p->max_blocks + kStrip - 1) / kStrip);
   constexpr int kStep = kForkThreads / kStrip;
-  if (p->slots <= kStep) hipLaunchKernelGGL((fork_tables_kernel<1>), grid, block, 0, st, *p);
-  else hipLaunchKernelGGL((fork_tables_kernel<kForkSlots / kStep>), grid, block, 0, st, *p);
-  hipLaunchKernelGGL(fork_pages_kernel, dim3(1), block, 0, st, *p);
+  if (p->slots <= kStep) hipLaunchKernelGGL(fork_tables_kernel<1>, grid, block, 0, st, *p);
+  else hipLaunchKernelGGL(fork_tables_kernel<kForkSlots / kStep>, grid, block, 0, st, *p);
+  hipLaunchKernelGGL(fork_pages_kernel<false>, dim3(1), block, 0, st, *p);
   return hipGetLastError();
 }
 
