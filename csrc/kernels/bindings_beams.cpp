@@ -215,6 +215,7 @@ void state_reorder(at::TensorList states, const Tensor& parents, int64_t width) 
     TORCH_CHECK(row * t.element_size() % 2 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 2 == 0 &&
                     (S == 1 || t.stride(0) * t.element_size() % 2 == 0) && row * t.element_size() < INT_MAX - (1 << 16),
                 "a slot's state must have an even number of bytes, under 2 GiB");
+    for (const Tensor& u : states) TORCH_CHECK(&u == &t || u.data_ptr() != t.data_ptr() || u.numel() == 0, "a state is listed twice");
   }
   if (S == 0) return;
   const c10::DeviceGuard guard(parents.device());

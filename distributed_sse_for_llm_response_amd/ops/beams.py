@@ -77,8 +77,8 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
 
 
 def state_reorder(states, parents, width: int):
-    """In every tensor of `states` ([slots, ..], any type, a slot's part contiguous), slot s takes what slot parents[s] held, in
-    place and for all slots at once.  parents [slots] int32 stay within their group of `width` slots; a slot whose parent is itself,
+    """In every tensor of `states` ([slots, ..], any type, a slot's part contiguous, no two of them overlapping), slot s takes what
+    slot parents[s] held, in place and for all slots at once.  parents [slots] int32 stay within their group of `width` slots; a slot whose parent is itself,
     or lies outside its group (an ended slot's -1), stays as it is."""
     if _hip(parents):
         torch.ops.dsse.state_reorder(states, parents, width)

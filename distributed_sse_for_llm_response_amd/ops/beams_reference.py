@@ -169,6 +169,7 @@ def state_reorder(states, parents, width):
         if t.numel():
             _need(t[0].is_contiguous() and (S == 1 or t.stride(0) >= t[0].numel()), "a slot's state must be contiguous")
             _need(t[0].numel() * t.element_size() % 2 == 0, "a slot's state must have an even number of bytes, under 2 GiB")
+            _need(sum(u.data_ptr() == t.data_ptr() and u.numel() > 0 for u in states) == 1, "a state is listed twice")
     src = [q if q // width == s // width and q >= 0 else s for s, q in enumerate(parents.tolist())]
     for t in states:
         t.copy_(t.clone()[torch.tensor(src, dtype=torch.long)])

@@ -160,7 +160,7 @@ def test_reorder_and_refusals():
     assert t[:, 0].tolist() == [2, 0, 4, 8, 8, 10] and h.tolist() == [1, 0, 2, 4, 4, 5]
     p = torch.arange(6, dtype=i32)
     for states, width in (([t], 4), ([t[:5]], 3), ([torch.zeros(6, 3, dtype=torch.uint8)], 3), ([torch.zeros(6, 4, 2).transpose(1, 2)], 3),
-                          ([torch.zeros(1, 4).expand(6, 4)], 3), ([t], 0), ([t], 33)):
+                          ([torch.zeros(1, 4).expand(6, 4)], 3), ([t], 0), ([t], 33), ([t, h, t], 3)):
         with pytest.raises(RuntimeError):
             ops.state_reorder(states, p, width)
     with pytest.raises(RuntimeError):

@@ -313,6 +313,77 @@ def test_attention_graph_and_stream(gpu):
             assert torch.equal(o, want)
 
 
+@pytest.mark.parametrize("width,hq,hkv", [(16, 16, 1), (32, 10, 1), (7, 16, 1)])
+def test_attention_many_columns(gpu, width, hq, hkv):
+    """More (beam, head) columns than one workgroup holds, and a last tile that is not full."""
+    gen = torch.Generator().manual_seed(width)
+    _attend(gpu, gen, [64 + 5 * s for s in range(width)], [2], width, hq, hkv)
+
+
+@pytest.mark.parametrize("width,hq", [(2, 16), (4, 32)])
+def test_attention_far_pages(gpu, width, hq):
+    """Pages beyond 2^31 elements and 2^32 bytes of a pool."""
+    gen = torch.Generator().manual_seed(width)
+    lens, common = [100 + s for s in range(width)], [2]
+    bt, small = _tables(gen, lens, common, width)
+    k, v = _cache(gen, small, 8, "cpu")
+    pages = 2 ** 31 // (8 * 32 * 128) + 64
+    bk = torch.zeros(pages, 8, 32, 128, dtype=torch.bfloat16, device=gpu)
+    bv = torch.zeros(pages, 8, 128, 32, dtype=torch.bfloat16, device=gpu)
+    far = pages - 1 - torch.arange(small)
+    bk[far], bv[far] = k.to(gpu), v.to(gpu)
+    q = torch.randn(width, hq, 128, generator=gen).to(torch.bfloat16).to(gpu)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    sh = torch.tensor(common, dtype=torch.int32, device=gpu)
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    ops.beam_attention(q, k.to(gpu), v.to(gpu), bt.to(gpu), ctx, sh, a, width)
+    ops.beam_attention(q, bk, bv, far[bt.long()].to(torch.int32).to(gpu), ctx, sh, b, width)
+    assert torch.equal(a, b) and bool(a.any())
+
+
+def test_attention_entries_that_are_no_pages(gpu):
+    """Ids outside the cache read page 0."""
+    gen = torch.Generator().manual_seed(8)
+    for width in (4, 8):  # pages to registers, pages through LDS
+        k, v = _cache(gen, 4, 2, gpu)
+        q = torch.randn(width, 8, 128, generator=gen).to(torch.bfloat16).to(gpu)
+        bad = torch.tensor([[1, 10 ** 6, 2, -3]] * width, dtype=torch.int32, device=gpu)
+        good = torch.tensor([[1, 0, 2, 0]] * width, dtype=torch.int32, device=gpu)
+        ctx = torch.full((width,), 128, dtype=torch.int32, device=gpu)
+        for shared in (0, 3):
+            sh = torch.tensor([shared], dtype=torch.int32, device=gpu)
+            a, b = torch.zeros_like(q), torch.zeros_like(q)
+            ops.beam_attention(q, k, v, bad, ctx, sh, a, width)
+            ops.beam_attention(q, k, v, good, ctx, sh, b, width)
+            assert torch.equal(a, b)
+
+
+def test_two_streams(gpu):
+    """Calls of every op on two streams at once, each with its own tensors: work areas are the calls' own."""
+    gen = torch.Generator().manual_seed(10)
+    sides = []
+    for n in (200, 333):
+        args, dsh, out = _attend(gpu, gen, [n, n + 9, n - 5, n + 1], [4], 4, 8, 2)
+        logits = _logits(gen, 4, 30000, torch.float32)
+        scores = _scores(gen, logits, 1, 4, 3)
+        sides.append((args, dsh, out, logits.to(gpu), scores, _select(gpu, logits.to(gpu), scores, 8)[0]))
+    streams = [torch.cuda.Stream() for _ in sides]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for st, (args, dsh, out, logits, scores, _) in zip(streams, sides):
+            with torch.cuda.stream(st):
+                o = torch.zeros_like(out)
+                ops.beam_attention(*args, dsh, o, 4)
+                t = (torch.zeros(1, 8, device=gpu), torch.zeros(1, 8, device=gpu, dtype=torch.int32), torch.zeros(1, 8, device=gpu, dtype=torch.int32))
+                ops.beam_select(logits, scores.to(gpu), *t)
+                got.append((o, t))
+    torch.cuda.synchronize()
+    for i, (o, t) in enumerate(got):
+        assert torch.equal(o, sides[i % 2][2])
+        _same_choice(sides[i % 2][5], [x.cpu() for x in t])
+
+
 # ---------------------------------------------------------------------------------------------------------------- forks
 def _fork_state(gen, lens, common, width, spare, M=None):
     bt, used = _tables(gen, lens, common, width, extra=2)
@@ -419,6 +490,23 @@ def test_fork_many_slots_and_pages(gpu):
     _fork(gpu, state, refs, parents, [torch.randn(1, refs.numel(), 8, generator=gen)])
 
 
+def test_fork_far_pages(gpu):
+    """A pool beyond 2^32 bytes, its layers strided."""
+    pages = 70000
+    pool = torch.zeros(2, pages + 7, 16384, dtype=torch.float32, device=gpu)[:, :pages]
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    refs = torch.ones(pages, dtype=torch.int32, device=gpu)
+    refs[pages - 2] = 0
+    refs[pages - 1] = 2
+    pool[:, pages - 1] = torch.randn(2, 16384, device=gpu)
+    bt, copies, starved = t([pages - 1], [0]), torch.zeros(2, 2, dtype=torch.int32, device=gpu), t(5)
+    held, lens = t(1, 0), t(31, 0)
+    refs[pages - 1] = 1
+    ops.page_fork(bt, held, lens, t(0, 0), refs, copies, starved, [pool])
+    assert copies.tolist() == [[pages - 1, pages - 2], [-1, -1]] and bt.tolist() == [[pages - 2], [pages - 1]] and int(starved) == 0
+    assert torch.equal(pool[:, pages - 2], pool[:, pages - 1]) and bool(pool[:, pages - 2].any()) and not bool(pool[:, : pages - 2].any())
+
+
 def test_fork_many_pools_and_a_graph(gpu):
     gen = torch.Generator().manual_seed(14)
     state, refs = _fork_state(gen, [40, 45, 50, 55], [1], 4, 40)
@@ -483,6 +571,73 @@ def test_reorder_views_and_many(gpu):
         assert torch.equal(a, b.cpu())
     assert torch.equal(dw.cpu(), wide)
     ops.state_reorder([], parents.to(gpu), 3)
+
+
+def test_reorder_far_slots(gpu):
+    """Slots beyond 2^32 bytes of a state."""
+    big = torch.zeros(5, 2 ** 28 + 4, device=gpu)
+    big[4, -3:] = 2.0
+    big[1, :2] = 3.0
+    ops.state_reorder([big], torch.tensor([4, 1, 2, 4, 1], dtype=torch.int32, device=gpu), 5)
+    want = [(0, 2), (3, 0), (0, 0), (0, 2), (3, 0)]
+    assert [(float(big[s, 0]), float(big[s, -1])) for s in range(5)] == want and float(big.sum()) == 2 * 3 * 2 + 2 * 2 * 3
+
+
+def test_refusals(gpu):
+    """What the CPU tests refuse, the bindings refuse too; and what only they can tell."""
+    import test_beams as cpu
+
+    i32 = dict(dtype=torch.int32, device=gpu)
+    b = dict(dtype=torch.bfloat16, device=gpu)
+    x, s = torch.zeros(4, 9, device=gpu), torch.zeros(2, 2, device=gpu)
+    o = [t.to(gpu) for t in cpu._outs(2, 3)]
+    for change in (dict(logits=x.half()), dict(logits=x.t().contiguous().t()), dict(logits=x[:3]), dict(scores=s.double()), dict(scores=s.cpu()),
+                   dict(scores=s.view(1, 4)), dict(out_rows=o[1].long()), dict(out_tokens=o[2][:, :2].contiguous()),
+                   dict(out_scores=torch.zeros(2, 65, device=gpu)), dict(eos_id=9), dict(eos_id=-2), dict(end_scores=torch.zeros(2, 2, device=gpu)),
+                   dict(end_scores=torch.zeros(2, 3, device=gpu), eos_id=1), dict(logits=x[:, :0]), dict(logits=x[:1].expand(4, 9))):
+        with pytest.raises(RuntimeError):
+            ops.beam_select(**{**dict(logits=x, scores=s, out_scores=o[0], out_rows=o[1], out_tokens=o[2], eos_id=-1, end_scores=None), **change})
+    a = dict(q=torch.zeros(4, 8, 128, **b), k_cache=torch.zeros(3, 2, 32, 128, **b), v_cache=torch.zeros(3, 2, 128, 32, **b),
+             block_tables=torch.zeros(4, 2, **i32), ctx_len=torch.ones(4, **i32), shared=torch.zeros(2, **i32), out=torch.zeros(4, 8, 128, **b),
+             width=2)
+    ops.beam_attention(**a)
+    odd = torch.zeros(4 * 8 * 128 + 1, **b)[1:].view(4, 8, 128)
+    for change in (dict(q=a["q"].float()), dict(q=a["q"][:, :, :64].contiguous()), dict(out=a["out"][:3]), dict(v_cache=a["k_cache"]), dict(width=3),
+                   dict(width=0), dict(width=33), dict(shared=torch.zeros(4, **i32)), dict(ctx_len=torch.ones(3, **i32)), dict(ctx_len=a["ctx_len"].cpu()),
+                   dict(block_tables=torch.zeros(4, 2, device=gpu, dtype=torch.int64)), dict(block_tables=torch.zeros(4, 4, **i32)[:, ::2]),
+                   dict(q=torch.zeros(4, 34, 128, **b), out=torch.zeros(4, 34, 128, **b)), dict(q=odd), dict(k_cache=a["k_cache"][:0], v_cache=a["v_cache"][:0])):
+        with pytest.raises(RuntimeError):
+            ops.beam_attention(**{**a, **change})
+    f = {k: [t.to(gpu) for t in v] if k == "pools" else v.to(gpu) for k, v in cpu._fork_args().items()}
+    ops.page_fork(**f)
+    far = torch.zeros(2 * 9 * 4 + 1, device=gpu)[1:].view(2, 9, 4)
+    for change in (dict(held=f["held"].long()), dict(lens=f["lens"][:3]), dict(parents=f["parents"][:3]), dict(copies=torch.zeros(4, **i32)),
+                   dict(starved=torch.zeros(2, **i32)), dict(refs=f["refs"][:0]), dict(pools=[torch.zeros(2, 8, 4, device=gpu)]),
+                   dict(pools=[torch.zeros(2, 9, 3, device=gpu)]), dict(pools=[torch.zeros(9, 4, device=gpu)]), dict(pools=[far]),
+                   dict(pools=[torch.zeros(2, 9, 4, 2, device=gpu)[..., 0]]), dict(pools=[torch.zeros(2, 9, 4)]),
+                   dict(pools=[torch.zeros(2, 9, 8, device=gpu)[:, :, :4]]), dict(block_tables=f["block_tables"].t())):
+        with pytest.raises(RuntimeError):
+            ops.page_fork(**{**f, **change})
+    t, p = torch.zeros(6, 2, device=gpu), torch.arange(6, **i32)
+    for states, width in (([t], 4), ([t[:5]], 3), ([torch.zeros(6, 3, dtype=torch.uint8, device=gpu)], 3), ([t.cpu()], 3), ([t, t], 3),
+                          ([torch.zeros(6, 4, 2, device=gpu).transpose(1, 2)], 3), ([torch.zeros(1, 4, device=gpu).expand(6, 4)], 3), ([t], 0), ([t], 33)):
+        with pytest.raises(RuntimeError):
+            ops.state_reorder(states, p, width)
+    with pytest.raises(RuntimeError):
+        ops.state_reorder([t], p.long(), 3)
+    torch.cuda.synchronize()
+
+
+def test_nothing_to_do(gpu):
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=gpu)  # noqa: E731
+    ops.beam_select(torch.zeros(0, 9, device=gpu), torch.zeros(0, 2, device=gpu), torch.zeros(0, 3, device=gpu), z(0, 3), z(0, 3))
+    e = torch.zeros(0, 8, 128, dtype=torch.bfloat16, device=gpu)
+    ops.beam_attention(e, torch.zeros(1, 2, 32, 128, dtype=torch.bfloat16, device=gpu), torch.zeros(1, 2, 128, 32, dtype=torch.bfloat16, device=gpu),
+                       z(0, 2), z(0), z(0), e.clone(), 4)
+    ops.beam_shared(z(0, 2), z(0), 4, z(0))
+    ops.page_fork(z(0, 2), z(0), z(0), z(0), z(3), z(0, 2), z(1))
+    ops.state_reorder([torch.zeros(0, 4, device=gpu)], z(0), 4)
+    torch.cuda.synchronize()
 
 
 def test_reorder_caches(gpu):
