@@ -15,7 +15,7 @@
 namespace dsse {
 namespace {
 
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 512;
 constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kGather = 1024;  // candidates that LDS holds; a chunk or group with more that reach the bound (many equal logits, the best
                                // ones all in a few threads) is walked K times instead
@@ -87,22 +87,28 @@ DEV V bound_of_lanes(V mine, int K, V* all, int* rank) {
   const unsigned long long who = __ballot(rank[lane] == K - 1);
   return lane_value(v, __ffsll(who) - 1);
 }
-// The same with a bucket per thread: nearer for many candidates, and for lists that are in order
+// The same with 128 buckets, where 64 would let too much through: 1.4 K for K = 64
 template <typename V>
-DEV V bound_of_threads(V mine, int K, V* all, int* rank) {
+DEV V bound_of_many(V mine, int K, V* all, int* rank) {
+  constexpr int kBuckets = 128, kParts = kSelThreads / kBuckets, kEach = kBuckets / kParts;
+  const int b = threadIdx.x % kBuckets, part = threadIdx.x / kBuckets;
   all[threadIdx.x] = mine;
-  if (threadIdx.x == 0) rank[0] = -1;
+  if (part == 0) rank[b] = 0;
   __syncthreads();
-  int n = 0;
+  V v = all[b];
+#pragma unroll
+  for (int k = 1; k < kParts; ++k) v = all[b + k * kBuckets] > v ? all[b + k * kBuckets] : v;
+  __syncthreads();
+  if (part == 0) all[b] = v;
+  __syncthreads();
+  int n = 0;  // buckets before this one, a part of them per thread; of equal ones the lower is before
 #pragma unroll 8
-  for (int i = 0; i < kSelThreads; ++i) n += all[i] > mine ? 1 : 0;
-  if (n < K) atomicMax(&rank[0], n);  // of the buckets with fewer than K above them, the lowest: equal ones have the same number
+  for (int i = part * kEach; i < part * kEach + kEach; ++i) n += all[i] > v || (all[i] == v && i < b) ? 1 : 0;
+  atomicAdd(&rank[b], n);
   __syncthreads();
-  const bool is = n == rank[0];
+  if (part == 0 && rank[b] == K - 1) all[kBuckets] = v;
   __syncthreads();
-  if (is) all[0] = mine;
-  __syncthreads();
-  return all[0];
+  return all[kBuckets];
 }
 
 // Q: 16-byte pieces of a thread.  A row is whole pieces at 16-byte addresses and the few elements before and behind them, which go
@@ -112,7 +118,7 @@ __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectPar
   constexpr int N = Piece<T>::N;
   __shared__ float s_max[kSelWaves], s_sum[kSelWaves];
   __shared__ float bucket[kSelThreads];
-  __shared__ int rank[64], count;
+  __shared__ int rank[128], count;
   __shared__ uint64_t got[kGather];
   const int row = blockIdx.y, c = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectPar
   const float top = wave_max(ref);
   sum = wave_sum(sum * exp_below(ref, top));
   if (lane == 0) s_max[wave] = top, s_sum[wave] = sum;
-  const float bound = p.K <= 32 ? bound_of_lanes(m, p.K, bucket, rank) : bound_of_threads(m, p.K, bucket, rank);
+  const float bound = p.K <= 32 ? bound_of_lanes(m, p.K, bucket, rank) : bound_of_many(m, p.K, bucket, rank);
   if (threadIdx.x == 0) {
     float all = s_max[0], s = 0.f;
 #pragma unroll
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
   __shared__ float top[kBeamWidth];
   __shared__ double bucket[kSelThreads];
   __shared__ Pick got[kGather];
-  __shared__ int rank[64], count, open[kHeld * kSelThreads], nopen;
+  __shared__ int rank[128], count, open[kHeld * kSelThreads], nopen;
   const int g = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) count = nopen = 0;
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
   };
   double best = -INFINITY;
   each([&](const Pick& c, int, int) { best = c.s > best ? c.s : best; });
-  const double bound = p.K <= 32 ? bound_of_lanes(best, p.K, bucket, rank) : bound_of_threads(best, p.K, bucket, rank);
+  const double bound = p.K <= 32 ? bound_of_lanes(best, p.K, bucket, rank) : bound_of_many(best, p.K, bucket, rank);
   auto gather = [&](const Pick& c) {
     const bool in = c.s >= bound && c.s > -INFINITY;
     if (in) {
