@@ -10,6 +10,9 @@
 //
 // Two candidates of different rows may be nearer to each other than 32 bits of a score of tens tell, so scores are compared in 64
 // bits, and the exponentials' argument carries the error of log2(e): a row's log-sum is off by some 1e-8, not 1e-6.
+//
+// 64 groups of 8 rows of 131072 bf16 logits, 16 candidates: 36 us (3.7 TB/s), 29 without the selection, which the exponentials share the
+// vector units with; the merge 7.3.  One group of 4 rows of 32768 (fp32): 4.2 and 4.7 us, all latency.
 #include "api_beams.h"
 
 namespace dsse {
@@ -75,7 +78,7 @@ DEV V bound_of_lanes(V mine, int K, V* all, int* rank) {
   V v = all[lane];
 #pragma unroll
   for (int w = 1; w < kSelWaves; ++w) v = all[w * 64 + lane] > v ? all[w * 64 + lane] : v;
-  int n = 0;  // buckets before this one, a quarter of them per wave; of equal ones the lower lane is before
+  int n = 0;  // buckets before this one, some of them per wave; of equal ones the lower lane is before
 #pragma unroll
   for (int i = 0; i < 64 / kSelWaves; ++i) {
     const int l = wave * (64 / kSelWaves) + i;
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
       if (gather(c) && at == deep - 1 && deep < p.K) {
         const int o = atomicAdd(&nopen, 1);
         if (o < kHeld * kSelThreads) open[o] = list;
-        else count = kGather + 1;  // (more lists than threads' registers: all of them by place)
+        else count = kGather + 1;  // `got` has overflowed by then: place by place, below
       }
     });
   __syncthreads();

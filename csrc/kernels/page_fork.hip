@@ -9,7 +9,8 @@
 //           device knows.
 //
 // Beams of a request have the same pages but for the last few, so the first launch is two reads of the tables and few atomics; the
-// copies are what costs, two passes over each page.
+// copies are what costs, two passes over each page: 64x8 slots behind 4000 tokens 4.4 + 7.9 us for tables and pages, 16.9 for 89 MB of
+// copies (5.3 TB/s); 16x4 slots over 32 layers of keys and values 9.6 in one launch and 49 for 252 MB (5.1 TB/s).
 #include "api_beams.h"
 
 namespace dsse {
@@ -27,8 +28,8 @@ DEV int holders(const PageForkParams& p, int page) {
   return __hip_atomic_load(&p.refs[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// A workgroup's part of the tables, N entries of a thread; place(n, s, j): whether entry n is one, and which.  No entry outside of the
-// part is read or written: all columns of a slot are moved by themselves.
+// A workgroup's part of the tables, whole columns of it, N entries of a thread; place(n, s, j): whether entry n is one, and which.  A
+// column's entries come from the same column, so no other workgroup reads what this one writes.
 template <int N, typename P>
 DEV void move_entries(const PageForkParams& p, P place) {
   int next[N], old[N];

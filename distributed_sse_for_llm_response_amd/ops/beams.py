@@ -22,8 +22,8 @@ FORK_SLOTS = 2048
 def beam_select(logits, scores, out_scores, out_rows, out_tokens, eos_id: int = -1, end_scores=None):
     """The K best continuations of each group over its beams and the vocabulary.
 
-    logits [groups * width, V] (fp32 or bf16, rows may be strided), scores [groups, width] fp32 (log-probabilities of the beams so
-    far, -inf for a beam that is not in use).  A continuation's score is scores[w] + log softmax(logits[row])[token]; out_scores,
+    logits [groups * width, V] (fp32 or bf16, whole vocabularies, rows may be strided), scores [groups, width] fp32 (log-probabilities
+    of the beams so far, -inf for a beam that is not in use).  A continuation's score is scores[w] + log softmax(logits[row])[token]; out_scores,
     out_rows, out_tokens [groups, K] receive the K <= 64 best by (score descending, row, token ascending): the score, the row of
     `logits` it came from -- the slot whose pages and state go on -- and the token.  Equal logits of a row are ordered by token;
     scores are compared in 64 bits and returned in 32.  A token of logit -inf is no candidate, and neither is anything of a row whose
@@ -78,8 +78,8 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
 
 def state_reorder(states, parents, width: int):
     """In every tensor of `states` ([slots, ..], any type, a slot's part contiguous, no two of them overlapping), slot s takes what
-    slot parents[s] held, in place and for all slots at once.  parents [slots] int32 stay within their group of `width` slots; a slot whose parent is itself,
-    or lies outside its group (an ended slot's -1), stays as it is."""
+    slot parents[s] held, in place and for all slots at once.  parents [slots] int32 stay within their group of `width` slots; a slot
+    whose parent is itself, or lies outside its group (an ended slot's -1), stays as it is."""
     if _hip(parents):
         torch.ops.dsse.state_reorder(states, parents, width)
     else:
