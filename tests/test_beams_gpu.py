@@ -111,6 +111,19 @@ def test_select_more_than_gathered(gpu, dtype, groups, width, V, K):
     _same_choice(want, got)
 
 
+def test_select_more_lists_than_noted(gpu):
+    """A vocabulary so long that the merge cannot note every list that goes on: all rows equal, or one ahead."""
+    V, K = 1 << 23, 5
+    logits = torch.zeros(32, V, device=gpu, dtype=torch.bfloat16)
+    o = (torch.zeros(1, K, device=gpu), torch.zeros(1, K, device=gpu, dtype=torch.int32), torch.zeros(1, K, device=gpu, dtype=torch.int32))
+    for ahead in (0, 7):
+        scores = torch.zeros(1, 32, device=gpu)
+        scores[0, ahead] = 1.0 if ahead else 0.0
+        ops.beam_select(logits, scores, *o, 1)
+        assert o[1].tolist() == [[ahead] * K] and o[2].tolist() == [[0, 2, 3, 4, 5]]
+        assert float((o[0] - (scores[0, ahead] - math.log(V))).abs().max()) < LOG_SUM + 2.0 ** -23 * 16
+
+
 def test_select_what_is_not_finite(gpu):
     gen = torch.Generator().manual_seed(3)
     logits = _logits(gen, 12, 3000, torch.float32)
@@ -659,6 +672,57 @@ def test_reorder_caches(gpu):
 
 
 # ----------------------------------------------------------------------------------------------------------- all together
+def test_a_step_in_a_graph(gpu):
+    """Choice, fork, states, shared pages and attention of a step as one graph, replayed over its own results, against the same calls made
+    one by one on copies."""
+    gen = torch.Generator().manual_seed(21)
+    W, G, V, H = 4, 3, 3000, 2
+    S = W * G
+    state, refs = _fork_state(gen, [70 + 9 * (s // W) for s in range(S)], [2] * G, W, 60)
+    state[0] = torch.cat([state[0], torch.zeros(S, 6, dtype=torch.int32)], 1)
+    k, v = _cache(gen, refs.numel(), H, "cpu")
+
+    def make():
+        d = dict(bt=state[0], held=state[1], lens=state[2], refs=refs, k=k[None], v=v[None], state=torch.randn(S, 64, 3, generator=torch.Generator().manual_seed(1)),
+                 scores=-torch.arange(S, dtype=torch.float32).view(G, W) / 7, logits=torch.zeros(S, V), q=torch.zeros(S, 8, 128, dtype=torch.bfloat16),
+                 rows=torch.zeros(G, W, dtype=torch.int32), tokens=torch.zeros(G, W, dtype=torch.int32), copies=torch.zeros(S, 2, dtype=torch.int32),
+                 starved=torch.zeros(1, dtype=torch.int32), shared=torch.zeros(G, dtype=torch.int32), out=torch.zeros(S, 8, 128, dtype=torch.bfloat16),
+                 new=torch.zeros(G, W))
+        return {n: t.clone().to(gpu) for n, t in d.items()}
+
+    def step(d):
+        ops.beam_select(d["logits"], d["scores"], d["new"], d["rows"], d["tokens"], 2)
+        d["scores"].copy_(d["new"])
+        ops.page_fork(d["bt"], d["held"], d["lens"], d["rows"].view(-1), d["refs"], d["copies"], d["starved"], [d["k"], d["v"]])
+        ops.state_reorder([d["state"]], d["rows"].view(-1), W)
+        d["lens"].add_(1)
+        ops.beam_shared(d["bt"], d["lens"], W, d["shared"])
+        ops.beam_attention(d["q"], d["k"][0], d["v"][0], d["bt"], d["lens"], d["shared"], d["out"], W)
+
+    a, b = make(), make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(make())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(a)
+    for i in range(40):
+        gen = torch.Generator().manual_seed(100 + i)
+        logits, q = _logits(gen, S, V, torch.float32), torch.randn(S, 8, 128, generator=gen).to(torch.bfloat16)
+        for d in (a, b):
+            d["logits"].copy_(logits)
+            d["q"].copy_(q)
+        g.replay()
+        torch.cuda.synchronize()
+        step(b)
+        for n in a:
+            assert torch.equal(a[n], b[n]), (i, n)
+    assert int(a["starved"]) == 0 and len({tuple(t) for t in a["copies"].tolist()}) > 1
+
+
 def test_a_search(gpu):
     from test_beams import check_search, search
 
