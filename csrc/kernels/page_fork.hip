@@ -33,24 +33,26 @@ DEV int holders(const PageForkParams& p, int page) {
 template <int N, typename P>
 DEV void move_entries(const PageForkParams& p, P place) {
   int next[N], old[N];
+  bool given[N];  // the parent holds the entry, whatever its number: a slot never keeps a page that it has given up
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     int s, j;
     next[n] = old[n] = -1;
+    given[n] = false;
     if (!place(n, s, j)) continue;
     const int q = p.parents[s];
     if (q == s) continue;
     if (j < p.held[s]) old[n] = p.tables[(size_t)s * p.max_blocks + j];
-    if (goes_on(q, p.slots) && j < p.held[q]) next[n] = p.tables[(size_t)q * p.max_blocks + j];
+    if (goes_on(q, p.slots) && j < p.held[q]) next[n] = p.tables[(size_t)q * p.max_blocks + j], given[n] = true;
   }
   __syncthreads();  // the part is read: it may change
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     int s, j;
-    if (!place(n, s, j) || old[n] == next[n]) continue;  // most of the pages that beams of a request hold
+    if (!place(n, s, j) || (old[n] == next[n] && old[n] >= 0)) continue;  // most of the pages that beams of a request hold
     if ((unsigned)old[n] < (unsigned)p.pages) atomicSub(&p.refs[old[n]], 1);
     if ((unsigned)next[n] < (unsigned)p.pages) atomicAdd(&p.refs[next[n]], 1);
-    if (next[n] >= 0) p.tables[(size_t)s * p.max_blocks + j] = next[n];
+    if (given[n]) p.tables[(size_t)s * p.max_blocks + j] = next[n];
   }
 }
 

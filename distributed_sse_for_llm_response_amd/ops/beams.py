@@ -69,7 +69,8 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
     old page holds tokens already, (-1, -1) elsewhere, and the page is copied in every pool: `pools` are tensors [layers, pages, ..]
     (KVCache.pools() and its like), whole pages of whole 16-byte units.  A slot that finds no free page keeps what it has, shared:
     starved [1] counts those, and once pages are free a call with parents[s] = s serves them.  A slot whose max_blocks pages are
-    full needs none.  Entries of a table past the slot's pages stay as they were.  At most 2048 slots."""
+    full needs none.  Entries of a table past the slot's pages stay as they were; a
+    number that is no page goes along with the others, but counts nowhere and is copied nowhere.  At most 2048 slots."""
     if _hip(block_tables):
         torch.ops.dsse.page_fork(block_tables, held, lens, parents, refs, copies, starved, pools)
     else:

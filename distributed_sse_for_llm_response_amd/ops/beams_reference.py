@@ -121,15 +121,18 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
         if t.numel():
             _need(t[0, 0].is_contiguous() and t[0].is_contiguous(), "a pool's pages must be contiguous")
             _need(t[0, 0].numel() * t.element_size() % 16 == 0, "a pool's pages must start and end at 16 bytes")
+    P = refs.numel()  # an entry outside of the pool goes along with the others, but has no count
     before, had, size = block_tables.clone(), held.clamp(0, M).tolist(), lens.tolist()
     goes = [q if 0 <= q < S else -1 for q in parents.tolist()]
     for s, q in enumerate(goes):  # every slot gives its pages up and takes its parent's
         n = had[q] if q >= 0 else 0
         for page in before[s, :had[s]].tolist():
-            refs[page] -= 1
+            if 0 <= page < P:
+                refs[page] -= 1
         block_tables[s, :n] = before[q, :n]
         for page in before[q, :n].tolist():
-            refs[page] += 1
+            if 0 <= page < P:
+                refs[page] += 1
         held[s], lens[s] = n, size[q] if q >= 0 else 0
     counts = refs.clone()
     free = (counts == 0).nonzero()[:, 0].tolist()
@@ -140,6 +143,8 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
         if q < 0 or j >= M:
             continue
         page = int(block_tables[s, j]) if j < int(held[s]) else -1
+        if j < int(held[s]) and not 0 <= page < P:
+            continue
         followers = [t for t in range(S) if goes[t] == q]
         if page >= 0 and s == followers[-1] and int(counts[page]) == len(followers):
             continue

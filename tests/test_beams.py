@@ -269,3 +269,16 @@ def check_search(result):
 
 def test_a_search():
     check_search(search("cpu"))
+
+
+def test_fork_entries_that_are_no_pages():
+    """Ids outside the pool, negative ones too, are carried along and count nowhere."""
+    a = _fork_args(2, 4, 9)
+    a["block_tables"].copy_(torch.tensor([[3, 4, 5, 0], [-4, 10 ** 6, 6, 0]]))
+    a["held"].fill_(3)
+    a["lens"].fill_(70)
+    a["refs"].copy_(torch.tensor([0, 0, 0, 1, 1, 1, 1, 0, 0]))
+    a["parents"].fill_(1)
+    ops.page_fork(**a)
+    assert a["block_tables"].tolist() == [[-4, 10 ** 6, 0, 0], [-4, 10 ** 6, 6, 0]]
+    assert a["refs"].tolist() == [1, 0, 0, 0, 0, 0, 1, 0, 0] and a["copies"].tolist() == [[6, 0], [-1, -1]] and int(a["starved"]) == 0

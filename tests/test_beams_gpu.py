@@ -493,6 +493,18 @@ def test_fork_entries_that_are_no_pages(gpu):
     assert copies.tolist() == [[-1, -1], [-1, -1]] and all(torch.equal(a, b) for a, b in zip(pools, before))
 
 
+@pytest.mark.parametrize("columns", [4, 2000])
+def test_fork_takes_on_entries_that_are_no_pages(gpu, columns):
+    """Where the parent has such an id, its follower has it too, not the page that it gave up: one launch, and one for the tables."""
+    state, refs = _fork_state(torch.Generator().manual_seed(14), [70, 70], [0], 2, 5)
+    state[0] = torch.cat([state[0], torch.zeros(2, columns, dtype=torch.int32)], 1)[:, :columns].contiguous()
+    refs[int(state[0][1, 0])] = refs[int(state[0][1, 1])] = 0
+    state[0][1, 0], state[0][1, 1] = -4, 10 ** 6
+    for parents in ([1, 1], [1, 0], [0, 0]):
+        got = _fork(gpu, state, refs, parents, _pools(torch.Generator().manual_seed(15), refs.numel()))
+        assert got[0][0, :2].tolist() == state[0][parents[0], :2].tolist()
+
+
 def test_fork_many_slots_and_pages(gpu):
     gen = torch.Generator().manual_seed(13)
     S, W = 2048, 8
