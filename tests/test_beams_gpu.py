@@ -111,6 +111,22 @@ def test_select_more_than_gathered(gpu, dtype, groups, width, V, K):
     _same_choice(want, got)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [7, 1001, 50001])
+def test_select_rows_of_equal_logits_tie(gpu, V, dtype):
+    """Beams of the same logits and scores tie whatever addresses their rows have: the lowest row first, the scores the same bits."""
+    gen = torch.Generator().manual_seed(V)
+    row = torch.randn(V, generator=gen).clamp(-3, 3)
+    row[V // 2], row[V // 3] = 5.0, 4.0
+    G, W = 3, 8
+    logits = row.to(dtype).to(gpu).expand(G * W, V).contiguous()
+    o = torch.zeros(G, 16, device=gpu), torch.zeros(G, 16, dtype=torch.int32, device=gpu), torch.zeros(G, 16, dtype=torch.int32, device=gpu)
+    ops.beam_select(logits, torch.full((G, W), -0.7, device=gpu), *o)
+    for g in range(G):
+        assert o[1][g].tolist() == 2 * list(range(g * W, g * W + W)) and o[2][g].tolist() == W * [V // 2] + W * [V // 3]
+    assert bool((o[0].view(-1, W) == o[0][0].view(2, W)[:, :1].repeat(G, 1)).all())
+
+
 def test_select_more_lists_than_noted(gpu):
     """A vocabulary so long that the merge cannot note every list that goes on: all rows equal, or one ahead."""
     V, K = 1 << 23, 5
