@@ -427,7 +427,7 @@ extern "C" void dsse_beam_plan(dsse::BeamAttnParams* p) {
 extern "C" hipError_t dsse_beam_attention(const dsse::BeamAttnParams* p, hipStream_t st) {
   using namespace dsse;
   if (p->slots < 1 || p->width < 1 || p->width > kBeamWidth || p->slots % p->width || p->group < 1 || p->group > 16 || p->ns < 1 || p->no < 1 ||
-      p->ns + p->no > 64 || p->hkv > 65535)
+      p->ns + p->no > 64 || (int64_t)p->slots * p->hq > kBeamRows)
     return hipErrorInvalidValue;
   const int groups = p->slots / p->width;
   const int per = waves_of(p->tiles) / kOwnWaves;  // own walks of a workgroup

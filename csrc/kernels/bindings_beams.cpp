@@ -119,7 +119,7 @@ void beam_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cach
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == S && block_tables.size(1) >= 1 && block_tables.size(1) < (1 << 26),
               "block_tables must be [slots, max_blocks]");
   TORCH_CHECK(ctx_len.numel() == S && shared.numel() == groups, "ctx_len must be [slots], shared [groups]");
-  TORCH_CHECK(S * hq < (1 << 26) && hkv <= 65535, "too many rows");
+  TORCH_CHECK(S * hq <= dsse::kBeamRows, "at most ", dsse::kBeamRows, " slots times q heads");
   if (S == 0) return;
   TORCH_CHECK(aligned16(q.data_ptr()) && aligned16(k_cache.data_ptr()) && aligned16(v_cache.data_ptr()) && aligned16(out.data_ptr()),
               "q, caches and out must start at 16 bytes");
@@ -177,8 +177,9 @@ void page_fork(Tensor& block_tables, Tensor& held, Tensor& lens, const Tensor& p
     if (t.numel() == 0) continue;
     TORCH_CHECK(packed(t, 1) && (t.size(0) == 1 || t.stride(0) >= t.numel() / t.size(0)), "a pool's pages must be contiguous");
     const int64_t bytes = t.numel() / t.size(0) / pages * t.element_size();
-    TORCH_CHECK(bytes % 16 == 0 && bytes < INT_MAX && aligned16(t.data_ptr()) && (t.size(0) == 1 || t.stride(0) * t.element_size() % 16 == 0),
+    TORCH_CHECK(bytes % 16 == 0 && aligned16(t.data_ptr()) && (t.size(0) == 1 || t.stride(0) * t.element_size() % 16 == 0),
                 "a pool's pages must start and end at 16 bytes");
+    TORCH_CHECK(bytes <= dsse::kCopyPage, "a page of a pool's layer is at most 1 GiB");  // 32-bit offsets
   }
   if (S == 0) return;
   const c10::DeviceGuard guard(block_tables.device());
@@ -206,6 +207,7 @@ void state_reorder(at::TensorList states, const Tensor& parents, int64_t width) 
   const int64_t S = parents.numel();
   const int groups = beams(S, width);
   TORCH_CHECK(groups <= 65535, "at most 65535 groups");
+  int64_t bytes = 0;
   for (const Tensor& t : states) {
     on(t, parents, "state", false);
     TORCH_CHECK(t.dim() >= 1 && t.size(0) == S, "a state must be [slots, ..]");
@@ -215,8 +217,10 @@ void state_reorder(at::TensorList states, const Tensor& parents, int64_t width) 
     TORCH_CHECK(row * t.element_size() % 2 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 2 == 0 &&
                     (S == 1 || t.stride(0) * t.element_size() % 2 == 0) && row * t.element_size() < INT_MAX - (1 << 16),
                 "a slot's state must have an even number of bytes, under 2 GiB");
+    bytes += row * t.element_size();
     for (const Tensor& u : states) TORCH_CHECK(&u == &t || u.data_ptr() != t.data_ptr() || u.numel() == 0, "a state is listed twice");
   }
+  TORCH_CHECK(bytes <= dsse::kReorderBytes, "at most 32 GiB of a slot in all");
   if (S == 0) return;
   const c10::DeviceGuard guard(parents.device());
   const hipStream_t st = stream_of(parents);

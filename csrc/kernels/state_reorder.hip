@@ -62,15 +62,17 @@ extern "C" hipError_t dsse_state_reorder(const dsse::StateReorderParams* in, hip
     return hipErrorInvalidValue;
   if (in->slots == 0 || in->ntensors == 0) return hipSuccess;
   StateReorderParams p = *in;
-  int64_t blocks = 0;
+  int64_t bytes = 0;
+  int blocks = 0;
   for (int i = 0; i < p.ntensors; ++i) {
     if ((reinterpret_cast<uintptr_t>(p.t[i].base) | (uintptr_t)p.t[i].stride | (uintptr_t)p.t[i].bytes) % 2) return hipErrorInvalidValue;
-    p.t[i].first = (int)blocks;
+    bytes += p.t[i].bytes;
+    if (bytes > kReorderBytes) return hipErrorInvalidValue;
+    p.t[i].first = blocks;
     const int items = p.t[i].bytes / 16 + p.t[i].bytes % 16 / 4 + (p.t[i].bytes % 4 ? 1 : 0);
     blocks += (items + kReorderThreads - 1) / kReorderThreads;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   }
-  const dim3 grid((unsigned)blocks, p.slots / p.width), block(kReorderThreads);
+  const dim3 grid(blocks, p.slots / p.width), block(kReorderThreads);
   if (p.width <= 4) hipLaunchKernelGGL(state_reorder_kernel<4>, grid, block, 0, st, p);
   else if (p.width <= 8) hipLaunchKernelGGL(state_reorder_kernel<8>, grid, block, 0, st, p);
   else if (p.width <= 16) hipLaunchKernelGGL(state_reorder_kernel<16>, grid, block, 0, st, p);

@@ -22,14 +22,15 @@ FORK_SLOTS = 2048
 def beam_select(logits, scores, out_scores, out_rows, out_tokens, eos_id: int = -1, end_scores=None):
     """The K best continuations of each group over its beams and the vocabulary.
 
-    logits [groups * width, V] (fp32 or bf16, whole vocabularies, rows may be strided), scores [groups, width] fp32 (log-probabilities
-    of the beams so far, -inf for a beam that is not in use).  A continuation's score is scores[w] + log softmax(logits[row])[token]; out_scores,
-    out_rows, out_tokens [groups, K] receive the K <= 64 best by (score descending, row, token ascending): the score, the row of
-    `logits` it came from -- the slot whose pages and state go on -- and the token.  Equal logits of a row are ordered by token;
-    scores are compared in 64 bits and returned in 32.  A token of logit -inf is no candidate, and neither is anything of a row whose
-    score or log-sum is not finite (NaN or +inf among its logits, all of them -inf); places that nothing is left for hold -inf, -1,
-    -1.  eos_id >= 0: that token counts in the softmax but is not offered; end_scores [groups, width] (optional) receives each
-    beam's score with it."""
+    logits [groups * width, V] (fp32 or bf16, whole vocabularies, rows may be strided), scores [groups, width] fp32 (log-
+    probabilities of the beams so far, -inf for a beam that is not in use).  A continuation's score is scores[w] + log
+    softmax(logits[row])[token]; out_scores, out_rows, out_tokens [groups, K] receive the K <= 64 best by (score descending,
+    row, token ascending): the score, the row of `logits` it came from -- the slot whose pages and state go on -- and the token.
+    Equal logits of a row are ordered by token; scores are compared in 64 bits, over log-sums of 32-bit terms (rows of the same
+    logits have the same), and returned in 32.  A token of logit -inf is no candidate, and neither is anything of a row whose
+    score or log-sum is not finite (NaN or +inf among its logits, all of them -inf); places that nothing is left for hold -inf,
+    -1, -1. eos_id >= 0: that token counts in the softmax but is not offered; end_scores [groups, width] (optional) receives
+    each beam's score with it."""
     if _hip(logits):
         torch.ops.dsse.beam_select(logits, scores, out_scores, out_rows, out_tokens, eos_id, end_scores)
     else:
@@ -51,7 +52,7 @@ def beam_attention(q, k_cache, v_cache, block_tables, ctx_len, shared, out, widt
     q, out [slots, Hq, 128] bf16, k_cache [blocks, Hkv, 32, 128], v_cache [blocks, Hkv, 128, 32] (KVCache's pages), up to 16 q heads
     per key/value head; slot s attends to its ctx_len[s] keys (its own among them), and a slot of ctx_len 0 is idle: its row of out
     stays as it was.  The first shared[g] pages must be the same in the tables of group g's live slots (beam_shared); they are read
-    once for the group, the others once per slot.  0 is always right."""
+    once for the group, the others once per slot.  0 is always right.  At most 2^22 rows (slots times Hq)."""
     if _hip(q):
         torch.ops.dsse.beam_attention(q, k_cache, v_cache, block_tables, ctx_len, shared, out, width)
     else:
@@ -67,10 +68,10 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
     lens // 32) then becomes its own: the last of the slots that follow a parent keeps it if they alone hold it, the others -- and
     every slot that has no such page yet -- get the lowest free pages in slot order.  copies [slots, 2] receives (old, new) where the
     old page holds tokens already, (-1, -1) elsewhere, and the page is copied in every pool: `pools` are tensors [layers, pages, ..]
-    (KVCache.pools() and its like), whole pages of whole 16-byte units.  A slot that finds no free page keeps what it has, shared:
-    starved [1] counts those, and once pages are free a call with parents[s] = s serves them.  A slot whose max_blocks pages are
-    full needs none.  Entries of a table past the slot's pages stay as they were; a
-    number that is no page goes along with the others, but counts nowhere and is copied nowhere.  At most 2048 slots."""
+    (KVCache.pools() and its like), whole pages of whole 16-byte units, at most 1 GiB in a layer.  A slot that finds no free page
+    keeps what it has, shared: starved [1] counts those, and once pages are free a call with parents[s] = s serves them.  A slot
+    whose max_blocks pages are full needs none.  Entries of a table past the slot's pages stay as they were; a number that is no
+    page goes along with the others, but counts nowhere and is copied nowhere.  At most 2048 slots."""
     if _hip(block_tables):
         torch.ops.dsse.page_fork(block_tables, held, lens, parents, refs, copies, starved, pools)
     else:
@@ -78,9 +79,10 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
 
 
 def state_reorder(states, parents, width: int):
-    """In every tensor of `states` ([slots, ..], any type, a slot's part contiguous, no two of them overlapping), slot s takes what
-    slot parents[s] held, in place and for all slots at once.  parents [slots] int32 stay within their group of `width` slots; a slot
-    whose parent is itself, or lies outside its group (an ended slot's -1), stays as it is."""
+    """In every tensor of `states` ([slots, ..], any type, a slot's part contiguous and under 2 GiB, at most 32 GiB in all, no two
+    of them overlapping), slot s takes what slot parents[s] held, in place and for all slots at once.  parents [slots] int32 stay
+    within their group of `width` slots; a slot whose parent is itself, or lies outside its group (an ended slot's -1), stays as it
+    is."""
     if _hip(parents):
         torch.ops.dsse.state_reorder(states, parents, width)
     else:

@@ -8,7 +8,7 @@ import torch
 
 from .reference import PAGE, gather_kv
 
-BEAM_WIDTH, BEAM_KEEP, FORK_SLOTS = 32, 64, 2048
+BEAM_WIDTH, BEAM_KEEP, FORK_SLOTS, BEAM_ROWS = 32, 64, 2048, 1 << 22
 
 
 def _need(ok: bool, text: str) -> None:
@@ -93,6 +93,7 @@ def beam_attention(q, k_cache, v_cache, block_tables, ctx_len, shared, out, widt
     _need(v_cache.shape == (*k_cache.shape[:2], 128, PAGE), "v_cache must be [blocks, Hkv, 128, 32]")
     S, hq, hkv = q.shape[0], q.shape[1], k_cache.shape[1]
     _need(hkv >= 1 and hq >= 1 and hq % hkv == 0 and hq // hkv <= 16, "up to 16 q heads per key/value head, the same for each")
+    _need(S * hq <= BEAM_ROWS, f"at most {BEAM_ROWS} slots times q heads")
     G = _beams(S, width)
     _need(block_tables.dim() == 2 and block_tables.shape[0] == S and block_tables.shape[1] >= 1, "block_tables must be [slots, max_blocks]")
     _need(ctx_len.numel() == S and shared.numel() == G, "ctx_len must be [slots], shared [groups]")
@@ -121,6 +122,7 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
         if t.numel():
             _need(t[0, 0].is_contiguous() and t[0].is_contiguous(), "a pool's pages must be contiguous")
             _need(t[0, 0].numel() * t.element_size() % 16 == 0, "a pool's pages must start and end at 16 bytes")
+            _need(t[0, 0].numel() * t.element_size() <= 1 << 30, "a page of a pool's layer is at most 1 GiB")
     P = refs.numel()  # an entry outside of the pool goes along with the others, but has no count
     before, had, size = block_tables.clone(), held.clamp(0, M).tolist(), lens.tolist()
     goes = [q if 0 <= q < S else -1 for q in parents.tolist()]
@@ -173,8 +175,10 @@ def state_reorder(states, parents, width):
         _need(t.dim() >= 1 and t.shape[0] == S, "a state must be [slots, ..]")
         if t.numel():
             _need(t[0].is_contiguous() and (S == 1 or t.stride(0) >= t[0].numel()), "a slot's state must be contiguous")
-            _need(t[0].numel() * t.element_size() % 2 == 0, "a slot's state must have an even number of bytes, under 2 GiB")
+            _need(t[0].numel() * t.element_size() % 2 == 0 and t[0].numel() * t.element_size() < (1 << 31) - 1 - (1 << 16),
+                  "a slot's state must have an even number of bytes, under 2 GiB")
             _need(sum(u.data_ptr() == t.data_ptr() and u.numel() > 0 for u in states) == 1, "a state is listed twice")
+    _need(sum(t[0].numel() * t.element_size() for t in states if t.numel()) <= 1 << 35, "at most 32 GiB of a slot in all")
     src = [q if q // width == s // width and q >= 0 else s for s, q in enumerate(parents.tolist())]
     for t in states:
         t.copy_(t.clone()[torch.tensor(src, dtype=torch.long)])

@@ -282,3 +282,20 @@ def test_fork_entries_that_are_no_pages():
     ops.page_fork(**a)
     assert a["block_tables"].tolist() == [[-4, 10 ** 6, 0, 0], [-4, 10 ** 6, 6, 0]]
     assert a["refs"].tolist() == [1, 0, 0, 0, 0, 0, 1, 0, 0] and a["copies"].tolist() == [[6, 0], [-1, -1]] and int(a["starved"]) == 0
+
+
+def too_large(device):
+    """Calls that a limit of sizes refuses, of tensors that nothing reads."""
+    e, z = lambda *s: torch.empty(*s, dtype=torch.uint8, device=device), lambda *s: torch.zeros(*s, dtype=i32, device=device)
+    q = torch.empty((1 << 19) + 2, 8, 128, dtype=torch.bfloat16, device=device)
+    k, v = (torch.zeros(1, 8, *s, dtype=torch.bfloat16, device=device) for s in ((32, 128), (128, 32)))
+    many = e((1 << 31) - (1 << 17) + 100)
+    return [lambda: ops.page_fork(z(2, 1), z(2), z(2), z(2), z(1), z(2, 2), z(1), [e(1, 1, (1 << 30) + 16)]),
+            lambda: ops.state_reorder([many[None, 2 * i: many.numel() - 100 + 2 * i] for i in range(17)], z(1), 1),
+            lambda: ops.beam_attention(q, k, v, z(q.shape[0], 1), z(q.shape[0]), z(q.shape[0] // 2), q, 2)]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_sizes_past_the_limits(which):
+    with pytest.raises(RuntimeError, match="at most"):
+        too_large("cpu")[which]()

@@ -669,6 +669,34 @@ def test_refusals(gpu):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_sizes_past_the_limits(gpu, which):
+    import test_beams as cpu
+
+    with pytest.raises(RuntimeError, match="at most"):
+        cpu.too_large(gpu)[which]()
+
+
+def test_most_rows(gpu):
+    """Attention over 2^22 rows of one key each is that key's value; choice over 65535 rows is the same in every group."""
+    S, H = 1 << 18, 16
+    k, v = _cache(torch.Generator().manual_seed(3), 1, H, gpu)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=gpu)  # noqa: E731
+    q = torch.ones(S, H, 128, dtype=torch.bfloat16, device=gpu)
+    out = torch.zeros_like(q)
+    ops.beam_attention(q, k, v, z(S, 1), z(S) + 1, z(S), out, 1)
+    _, mine = gather_kv(k.cpu(), v.cpu(), torch.zeros(1, dtype=torch.int32), 1)
+    assert bool((out == mine[0].to(gpu)).all())
+    G, W = 13107, 5
+    logits = (torch.arange(W * 7, device=gpu).float() * 3 % 11).view(1, W, 7).expand(G, W, 7).reshape(G * W, 7).contiguous()
+    o = torch.zeros(G, 9, device=gpu), z(G, 9), z(G, 9)
+    ops.beam_select(logits, torch.zeros(G, W, device=gpu), *o)
+    one = torch.zeros(1, 9), torch.zeros(1, 9, dtype=torch.int32), torch.zeros(1, 9, dtype=torch.int32)
+    bref.beam_select(logits[:W].cpu(), torch.zeros(1, W), *one)
+    assert torch.equal(o[2].cpu(), one[2].expand(G, 9)) and bool((o[0] == o[0][0]).all())
+    assert torch.equal(o[1].cpu(), one[1] + W * torch.arange(G, dtype=torch.int32)[:, None])
+
+
 def test_nothing_to_do(gpu):
     z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=gpu)  # noqa: E731
     ops.beam_select(torch.zeros(0, 9, device=gpu), torch.zeros(0, 2, device=gpu), torch.zeros(0, 3, device=gpu), z(0, 3), z(0, 3))
