@@ -22,15 +22,15 @@ FORK_SLOTS = 2048
 def beam_select(logits, scores, out_scores, out_rows, out_tokens, eos_id: int = -1, end_scores=None):
     """The K best continuations of each group over its beams and the vocabulary.
 
-    logits [groups * width, V] (fp32 or bf16, whole vocabularies, rows may be strided), scores [groups, width] fp32 (log-
-    probabilities of the beams so far, -inf for a beam that is not in use).  A continuation's score is scores[w] + log
+    logits [groups * width, V] (fp32 or bf16, whole vocabularies, rows may be strided), scores [groups, width] fp32
+    (log-probabilities of the beams so far, -inf for a beam that is not in use).  A continuation's score is scores[w] + log
     softmax(logits[row])[token]; out_scores, out_rows, out_tokens [groups, K] receive the K <= 64 best by (score descending,
     row, token ascending): the score, the row of `logits` it came from -- the slot whose pages and state go on -- and the token.
     Equal logits of a row are ordered by token; scores are compared in 64 bits, over log-sums of 32-bit terms (rows of the same
     logits have the same), and returned in 32.  A token of logit -inf is no candidate, and neither is anything of a row whose
     score or log-sum is not finite (NaN or +inf among its logits, all of them -inf); places that nothing is left for hold -inf,
-    -1, -1. eos_id >= 0: that token counts in the softmax but is not offered; end_scores [groups, width] (optional) receives
-    each beam's score with it."""
+    -1, -1.  eos_id >= 0: that token counts in the softmax but is not offered; end_scores [groups, width] (optional) receives
+    each beam's score with it.  Outputs overlap neither the inputs nor each other, but with K = width out_scores may be `scores`."""
     if _hip(logits):
         torch.ops.dsse.beam_select(logits, scores, out_scores, out_rows, out_tokens, eos_id, end_scores)
     else:

@@ -44,6 +44,18 @@ def test_select_orders_equal_scores():
     assert o[1].tolist() == [[1, 1, 1, 1, 2]] and o[2].tolist() == [[0, 1, 2, 3, 0]]
 
 
+def test_select_scores_in_place():
+    """The new scores may take the old ones' place."""
+    gen = torch.Generator().manual_seed(31)
+    x, s = torch.randn(12, 900, generator=gen), -torch.rand(3, 4, generator=gen)
+    apart = torch.zeros(3, 4), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 4, dtype=torch.int32)
+    end, end2 = torch.zeros(3, 4), torch.zeros(3, 4)
+    ops.beam_select(x, s, *apart, 5, end)
+    rows, tokens = torch.zeros_like(apart[1]), torch.zeros_like(apart[2])
+    ops.beam_select(x, s, s, rows, tokens, 5, end2)
+    assert torch.equal(s, apart[0]) and torch.equal(rows, apart[1]) and torch.equal(tokens, apart[2]) and torch.equal(end, end2)
+
+
 def test_select_refusals():
     x, s, o = torch.zeros(4, 9), torch.zeros(2, 2), _outs(2, 3)
     bad = [dict(logits=x.half()), dict(logits=x.t().contiguous().t()), dict(logits=x[:3]), dict(scores=s.double()), dict(scores=s.view(1, 4)),

@@ -127,6 +127,18 @@ def test_select_rows_of_equal_logits_tie(gpu, V, dtype):
     assert bool((o[0].view(-1, W) == o[0][0].view(2, W)[:, :1].repeat(G, 1)).all())
 
 
+def test_select_scores_in_place(gpu):
+    """The new scores may take the old ones' place."""
+    gen = torch.Generator().manual_seed(31)
+    x, s = torch.randn(12, 900, generator=gen).to(gpu), -torch.rand(3, 4, generator=gen).to(gpu)
+    apart = torch.zeros(3, 4, device=gpu), torch.zeros(3, 4, dtype=torch.int32, device=gpu), torch.zeros(3, 4, dtype=torch.int32, device=gpu)
+    end, end2 = torch.zeros(3, 4, device=gpu), torch.zeros(3, 4, device=gpu)
+    ops.beam_select(x, s, *apart, 5, end)
+    rows, tokens = torch.zeros_like(apart[1]), torch.zeros_like(apart[2])
+    ops.beam_select(x, s, s, rows, tokens, 5, end2)
+    assert torch.equal(s, apart[0]) and torch.equal(rows, apart[1]) and torch.equal(tokens, apart[2]) and torch.equal(end, end2)
+
+
 def test_select_more_lists_than_noted(gpu):
     """A vocabulary so long that the merge cannot note every list that goes on: all rows equal, or one ahead."""
     V, K = 1 << 23, 5
