@@ -18,7 +18,7 @@
 // where one of 3 lets three: 2x16 beams of 31077 tokens 36 -> 28.6 us.
 //
 // Measured, walks + join: 8x8 beams of 32 heads over 8 and some 8300 tokens 60 + 5 us (5.6 TB/s in the walks), 2x16 of 16 over 4 and
-// 31077 29 + 5, 16x4 of 612 15 + 4.  Each beam's pages read by themselves are 6 times the bytes in the first case, 15 in the second.
+// 31077 29 to 33 + 5, 16x4 of 612 15 + 4.  Each beam's pages read by themselves are 6 times the bytes in the first case, 15 in the second.
 //
 // Statistics and sums in fp32; scores in base 2 with the scale folded in; weights rounded to bf16 for the second product, as in
 // paged_attention.

@@ -11,8 +11,8 @@
 // Two candidates of different rows may be nearer to each other than 32 bits of a score of tens tell, so scores are compared in 64
 // bits, and the exponentials' argument carries the error of log2(e): a row's log-sum is off by some 1e-8, not 1e-6.
 //
-// 64 groups of 8 rows of 131072 bf16 logits, 16 candidates: 36 us (3.7 TB/s), 29 without the selection, which the exponentials share the
-// vector units with; the merge 7.3.  One group of 4 rows of 32768 (fp32): 4.2 and 4.7 us, all latency.
+// 64 groups of 8 rows of 131072 bf16 logits, 16 candidates: 35 to 36 us (3.8 TB/s), 29 without the selection, which the exponentials share the
+// vector units with; the merge 7.3.  One group of 4 rows of 32768 (fp32): 4.4 and 4.6 us, all latency.
 #include "api_beams.h"
 
 namespace dsse {

@@ -4,7 +4,7 @@
 // In place without a copy on the side: a thread owns the same bytes of every slot of a group.  It loads what the group's slots
 // take, all loads before its first store, so it has read a slot before anyone overwrites it (only it touches these bytes).  A slot
 // that keeps its own state is neither read nor written; a source that several slots take is read from memory once, the further
-// loads hit the cache.  Bound by memory: each source read once, each changed slot written once (64 slots of 6 x 1 MB 99 us, 5.3 TB/s).
+// loads hit the cache.  Bound by memory: each source read once, each changed slot written once (64 slots of 6 x 1 MB 100 us, 5.3 TB/s).
 // 16 bytes a thread whatever the slots' alignment: 128 slots with tails of 9612 bytes beside 1 MB 298 us by words, 186 so.
 #include "api_beams.h"
 
