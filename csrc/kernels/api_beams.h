@@ -13,6 +13,8 @@ constexpr int kForkSlots = 2048;
 constexpr int kReorderLists = 96;  // tensors of one launch (24 bytes each of a kernel's arguments)
 constexpr int kCopyPools = 64;     // (32 bytes each)
 constexpr int kCopyPage = 1 << 30;     // bytes of a page in a layer: offsets past its end, of whole work items, stay in 32 bits
+constexpr int kCopyPiece = 1 << 14;    // bytes of a page that a workgroup copies at a time
+constexpr int kCopyPieces = 0x7fffffff;  // pieces of a fork's slots over all pools and layers: a launch counts them in 32 bits
 constexpr int kBeamRows = 1 << 22;     // (slot, q head) pairs of an attention: a grid's threads stay in 32 bits
 constexpr int64_t kReorderBytes = int64_t{1} << 35;  // bytes of a slot over all tensors: so do those of a launch
 

@@ -171,6 +171,7 @@ void page_fork(Tensor& block_tables, Tensor& held, Tensor& lens, const Tensor& p
   TORCH_CHECK(held.numel() == S && lens.numel() == S && parents.numel() == S, "held, lens and parents must be [slots]");
   TORCH_CHECK(copies.dim() == 2 && copies.size(0) == S && copies.size(1) == 2 && starved.numel() == 1, "copies must be [slots, 2], starved [1]");
   TORCH_CHECK(pages >= 1 && pages < (1 << 30), "refs must have a count per page");
+  int64_t pieces = 0;  // of a slot
   for (const Tensor& t : pools) {
     on(t, block_tables, "pool", false);
     TORCH_CHECK(t.dim() >= 3 && t.size(1) == pages, "a pool must be [layers, pages, ..]");
@@ -180,6 +181,8 @@ void page_fork(Tensor& block_tables, Tensor& held, Tensor& lens, const Tensor& p
     TORCH_CHECK(bytes % 16 == 0 && aligned16(t.data_ptr()) && (t.size(0) == 1 || t.stride(0) * t.element_size() % 16 == 0),
                 "a pool's pages must start and end at 16 bytes");
     TORCH_CHECK(bytes <= dsse::kCopyPage, "a page of a pool's layer is at most 1 GiB");  // 32-bit offsets
+    pieces += t.size(0) * ((bytes + dsse::kCopyPiece - 1) / dsse::kCopyPiece);
+    TORCH_CHECK(pieces <= dsse::kCopyPieces / std::max<int64_t>(S, 1), "pages of all slots, pools and layers are at most 2^31 - 1 pieces of 16 KiB");
   }
   if (S == 0) return;
   const c10::DeviceGuard guard(block_tables.device());

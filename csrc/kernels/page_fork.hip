@@ -197,11 +197,11 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
   }
 }
 
-// Work item: 16 KB of a page of a pool's layer, for one of the listed slots
+// Work item: 16 KB of a page of a pool's layer, for one of the listed slots; up to 2^31 - 1 of them, and a workgroup's step further
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(PageCopyParams p) {
-  const int total = p.list[0] * p.blocks;
-  for (int w = blockIdx.x; w < total; w += gridDim.x) {
-    const int slot = p.list[1 + w / p.blocks], b = w % p.blocks;
+  const unsigned blocks = p.blocks, total = p.list[0] * blocks;
+  for (unsigned w = blockIdx.x; w < total; w += gridDim.x) {
+    const int slot = p.list[1 + w / blocks], b = w % blocks;
     const int src = p.copies[2 * slot], dst = p.copies[2 * slot + 1];
     int i = 0;
     while (i + 1 < p.npools && b >= p.pool[i + 1].first) ++i;
@@ -241,13 +241,13 @@ extern "C" hipError_t dsse_page_copy(const dsse::PageCopyParams* in, hipStream_t
   using namespace dsse;
   if (in->slots < 1 || in->slots > kForkSlots || in->npools < 1 || in->npools > kCopyPools) return hipErrorInvalidValue;
   PageCopyParams p = *in;
-  constexpr int kBlock = kCopyThreads * kCopyUnits * 16;
+  static_assert(kCopyThreads * kCopyUnits * 16 == kCopyPiece, "a work item is a piece");
   int64_t blocks = 0;
   for (int i = 0; i < p.npools; ++i) {
-    p.pool[i].per = (p.pool[i].bytes + kBlock - 1) / kBlock;
+    p.pool[i].per = (p.pool[i].bytes + kCopyPiece - 1) / kCopyPiece;
     p.pool[i].first = (int)blocks;
     blocks += (int64_t)p.pool[i].per * p.pool[i].layers;
-    if (blocks * p.slots > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks * p.slots > kCopyPieces) return hipErrorInvalidValue;
   }
   p.blocks = (int)blocks;
   const int64_t most = blocks * p.slots;  // all slots copy

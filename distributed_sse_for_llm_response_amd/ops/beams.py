@@ -68,7 +68,8 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
     lens // 32) then becomes its own: the last of the slots that follow a parent keeps it if they alone hold it, the others -- and
     every slot that has no such page yet -- get the lowest free pages in slot order.  copies [slots, 2] receives (old, new) where the
     old page holds tokens already, (-1, -1) elsewhere, and the page is copied in every pool: `pools` are tensors [layers, pages, ..]
-    (KVCache.pools() and its like), whole pages of whole 16-byte units, at most 1 GiB in a layer.  A slot that finds no free page
+    (KVCache.pools() and its like), whole pages of whole 16-byte units, at most 1 GiB in a layer and, a page of
+    each slot in every pool and layer together, 2^31 - 1 pieces of 16 KiB.  A slot that finds no free page
     keeps what it has, shared: starved [1] counts those, and once pages are free a call with parents[s] = s serves them.  A slot
     whose max_blocks pages are full needs none.  Entries of a table past the slot's pages stay as they were; a number that is no
     page goes along with the others, but counts nowhere and is copied nowhere.  At most 2048 slots."""

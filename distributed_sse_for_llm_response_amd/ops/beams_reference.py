@@ -9,6 +9,7 @@ import torch
 from .reference import PAGE, gather_kv
 
 BEAM_WIDTH, BEAM_KEEP, FORK_SLOTS, BEAM_ROWS = 32, 64, 2048, 1 << 22
+COPY_PIECE, COPY_PIECES = 1 << 14, (1 << 31) - 1
 
 
 def _need(ok: bool, text: str) -> None:
@@ -117,12 +118,15 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
     _need(held.numel() == S and lens.numel() == S and parents.numel() == S, "held, lens and parents must be [slots]")
     _need(copies.shape == (S, 2) and starved.numel() == 1, "copies must be [slots, 2], starved [1]")
     _need(refs.numel() >= 1, "refs must have a count per page")
+    pieces = 0
     for t in pools:
         _need(t.dim() >= 3 and t.shape[1] == refs.numel(), "a pool must be [layers, pages, ..]")
         if t.numel():
             _need(t[0, 0].is_contiguous() and t[0].is_contiguous(), "a pool's pages must be contiguous")
             _need(t[0, 0].numel() * t.element_size() % 16 == 0, "a pool's pages must start and end at 16 bytes")
             _need(t[0, 0].numel() * t.element_size() <= 1 << 30, "a page of a pool's layer is at most 1 GiB")
+            pieces += t.shape[0] * -(-t[0, 0].numel() * t.element_size() // COPY_PIECE)
+            _need(S * pieces <= COPY_PIECES, "pages of all slots, pools and layers are at most 2^31 - 1 pieces of 16 KiB")
     P = refs.numel()  # an entry outside of the pool goes along with the others, but has no count
     before, had, size = block_tables.clone(), held.clamp(0, M).tolist(), lens.tolist()
     goes = [q if 0 <= q < S else -1 for q in parents.tolist()]

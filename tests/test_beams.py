@@ -311,3 +311,19 @@ def too_large(device):
 def test_sizes_past_the_limits(which):
     with pytest.raises(RuntimeError, match="at most"):
         too_large("cpu")[which]()
+
+
+def refused_fork(device):
+    """A fork with more pieces to copy than a launch counts, its state, and a copy of that."""
+    a = {k: v if k == "pools" else v.to(device) for k, v in _fork_args(S=2048, M=1, P=1).items()}
+    a["held"][0], a["lens"][0], a["refs"][0] = 1, 3, 1
+    a["parents"].zero_()
+    a["pools"] = [torch.zeros(1 << 20, 1, 16, dtype=torch.uint8, device=device)]
+    return a, {k: v.clone() for k, v in a.items() if k != "pools"}
+
+
+def test_fork_refuses_before_it_moves():
+    a, before = refused_fork("cpu")
+    with pytest.raises(RuntimeError, match="pieces"):
+        ops.page_fork(**a)
+    assert all(torch.equal(a[k], v) for k, v in before.items())

@@ -795,3 +795,13 @@ def test_a_search(gpu):
     from test_beams import check_search, search
 
     check_search(search(gpu))
+
+
+# ------------------------------------------------------------------------------------------------------ calls at the borders
+def test_fork_refuses_before_it_moves(gpu):
+    import test_beams as cpu
+
+    a, before = cpu.refused_fork(gpu)
+    with pytest.raises(RuntimeError, match="pieces"):
+        ops.page_fork(**a)
+    assert all(torch.equal(a[k], v) for k, v in before.items())
