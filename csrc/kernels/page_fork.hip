@@ -88,7 +88,7 @@ DEV int block_scan(int v, int* sh, int& total) {
 
 template <bool TABLES>
 __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams p) {
-  __shared__ int follow[kForkSlots], last[kForkSlots], fresh[kForkSlots], scan[kForkThreads / 64];
+  __shared__ int follow[kForkSlots], last[kForkSlots], fresh[kForkSlots], goes_to[kForkSlots], scan[kForkThreads / 64];
   constexpr int kPer = kForkSlots / kForkThreads;  // neighbouring slots of a thread
   const int s0 = threadIdx.x * kPer;
   if constexpr (TABLES) {
@@ -125,20 +125,38 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
     }
   }
   __syncthreads();  // lengths and page counts are read: they may change
-  int page[kPer], need = 0, mask = 0;
+  int page[kPer], shared_by[kPer], mask = 0, ask = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    page[i] = -1;
+    page[i] = shared_by[i] = goes_to[s0 + i] = -1;
     const int s = s0 + i, q = parent[i], j = len[i] / kBS;
     if (q < 0 || len[i] < 0 || j >= p.max_blocks) continue;
     if (j < held[i]) {
       page[i] = p.tables[(size_t)s * p.max_blocks + j];
       if ((unsigned)page[i] >= (unsigned)p.pages) { page[i] = -1; continue; }
-      if (last[q] == s && holders(p, page[i]) == follow[q]) continue;  // its followers alone hold it: the last one keeps it
+      goes_to[s] = page[i];
+      const int held_by = holders(p, page[i]);
+      if (held_by == follow[q]) {  // its followers alone hold it: the last one keeps it
+        if (last[q] == s) continue;
+      } else {
+        shared_by[i] = held_by, ask = 1;
+      }
     }
     mask |= 1 << i;
-    ++need;
   }
+  // Slots of several parents go on in one page where an earlier call found no free one.  That is rare, so all slots are looked through
+  // then: if they alone hold it, the last of them keeps it.
+  if (__syncthreads_or(ask)) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (shared_by[i] < 0) continue;
+      int n = 0, end = -1;
+      for (int t = 0; t < p.slots; ++t)
+        if (goes_to[t] == page[i]) ++n, end = t;
+      if (n == shared_by[i] && end == s0 + i) mask &= ~(1 << i);
+    }
+  }
+  const int need = __popc(mask);
   int wanted;
   int rank = block_scan(need, scan, wanted);
   // the lowest free pages, as many as are wanted

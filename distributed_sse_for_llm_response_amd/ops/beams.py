@@ -65,14 +65,15 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
     block_tables [slots, max_blocks], held [slots] (pages of a slot), lens [slots] (tokens of a slot), refs [pages] (holders of a
     page, 0 = free), all int32.  Every slot takes its parent's pages and length; a parent outside [0, slots) ends the slot: it holds
     nothing any more.  Pages that nobody holds are free from then on.  The page that a slot's next token goes to (number
-    lens // 32) then becomes its own: the last of the slots that follow a parent keeps it if they alone hold it, the others -- and
-    every slot that has no such page yet -- get the lowest free pages in slot order.  copies [slots, 2] receives (old, new) where the
-    old page holds tokens already, (-1, -1) elsewhere, and the page is copied in every pool: `pools` are tensors [layers, pages, ..]
-    (KVCache.pools() and its like), whole pages of whole 16-byte units, at most 1 GiB in a layer and, a page of
-    each slot in every pool and layer together, 2^31 - 1 pieces of 16 KiB.  A slot that finds no free page
-    keeps what it has, shared: starved [1] counts those, and once pages are free a call with parents[s] = s serves them.  A slot
-    whose max_blocks pages are full needs none.  Entries of a table past the slot's pages stay as they were; a number that is no
-    page goes along with the others, but counts nowhere and is copied nowhere.  At most 2048 slots."""
+    lens // 32) then becomes its own: of the slots that go on in one page (those of a parent; of several where an earlier call found
+    no free page) the last keeps it if they alone hold it, the others -- and every slot that has no such page yet -- get the lowest
+    free pages in slot order.  copies [slots, 2] receives (old, new) where the old page holds tokens already, (-1, -1) elsewhere, and
+    the page is copied in every pool: `pools` are tensors [layers, pages, ..] (KVCache.pools() and its like), whole pages of whole
+    16-byte units, at most 1 GiB in a layer and, a page of each slot in every pool and layer together, 2^31 - 1 pieces of 16 KiB.  A
+    slot that finds no free page keeps what it has, shared: starved [1] counts those, and once pages are free a call with parents[s]
+    = s serves them: as many as were starved are enough.  A slot whose max_blocks pages are full needs none.  Entries of a table past
+    the slot's pages stay as they were; a number that is no page goes along with the others, but counts nowhere and is copied
+    nowhere.  At most 2048 slots."""
     if _hip(block_tables):
         torch.ops.dsse.page_fork(block_tables, held, lens, parents, refs, copies, starved, pools)
     else:

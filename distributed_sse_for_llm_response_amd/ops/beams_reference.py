@@ -144,15 +144,16 @@ def page_fork(block_tables, held, lens, parents, refs, copies, starved, pools=()
     free = (counts == 0).nonzero()[:, 0].tolist()
     copies.fill_(-1)
     starved.zero_()
+    at = [int(lens[s]) // PAGE for s in range(S)]
+    goes_to = [int(block_tables[s, j]) if q >= 0 and 0 <= j < min(M, int(held[s])) else -1 for s, (q, j) in enumerate(zip(goes, at))]
     for s, q in enumerate(goes):
-        j = int(lens[s]) // PAGE
-        if q < 0 or j >= M:
+        j, page = at[s], goes_to[s]
+        if q < 0 or not 0 <= j < M:
             continue
-        page = int(block_tables[s, j]) if j < int(held[s]) else -1
         if j < int(held[s]) and not 0 <= page < P:
             continue
-        followers = [t for t in range(S) if goes[t] == q]
-        if page >= 0 and s == followers[-1] and int(counts[page]) == len(followers):
+        alike = [t for t in range(S) if goes_to[t] == page]
+        if page >= 0 and s == alike[-1] and int(counts[page]) == len(alike):
             continue
         if not free:
             starved += 1

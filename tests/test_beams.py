@@ -7,6 +7,7 @@ import torch
 
 from distributed_sse_for_llm_response_amd import ops
 from distributed_sse_for_llm_response_amd.engine import kv_cache
+from distributed_sse_for_llm_response_amd.ops import beams_reference as bref
 
 INF = math.inf
 i32 = torch.int32
@@ -327,3 +328,36 @@ def test_fork_refuses_before_it_moves():
     with pytest.raises(RuntimeError, match="pieces"):
         ops.page_fork(**a)
     assert all(torch.equal(a[k], v) for k, v in before.items())
+
+
+def starved_forks(sharers, free):
+    """One sequence of 5 tokens that `sharers` slots go on from without a free page, then `free` pages given back and the call that
+    serves them: its arguments, and what it has to leave."""
+    S, P = sharers + 1, sharers + 7
+    a = _fork_args(S, 3, P)
+    a["held"][0], a["lens"][0] = 1, 5
+    a["block_tables"][0, 0] = 1
+    a["refs"].fill_(1)
+    a["parents"].copy_(torch.tensor([0] * sharers + [-1]))
+    bref.page_fork(**a)
+    assert int(a["starved"]) == sharers - 1 and a["refs"].tolist() == [1, sharers] + [1] * (P - 2)
+    a["refs"][3: 3 + free] = 0
+    a["parents"].copy_(torch.tensor(list(range(sharers)) + [-1]))
+    a["pools"] = [torch.arange(2 * P * 4.0).view(2, P, 4)]
+    served = min(free, sharers - 1)
+    pages = [3 + s for s in range(served)] + [1] * (sharers - served)
+    refs = [1, sharers - served] + [1] * (P - 2)
+    refs[3 + served: 3 + free] = [0] * (free - served)
+    return a, dict(block_tables=[[p, 0, 0] for p in pages] + [[0, 0, 0]], refs=refs, starved=[sharers - 1 - served],
+                   copies=[[1, 3 + s] for s in range(served)] + [[-1, -1]] * (S - served), held=[1] * sharers + [0],
+                   lens=[5] * sharers + [0])
+
+
+@pytest.mark.parametrize("sharers", [2, 3, 5])
+@pytest.mark.parametrize("free", [0, 1, 2, 4])
+def test_fork_serves_the_starved_with_as_many_pages(sharers, free):
+    a, want = starved_forks(sharers, free)
+    ops.page_fork(**a)
+    assert {k: a[k].tolist() for k in want} == want
+    for old, new in want["copies"]:
+        assert old < 0 or torch.equal(a["pools"][0][:, new], a["pools"][0][:, old])

@@ -805,3 +805,33 @@ def test_fork_refuses_before_it_moves(gpu):
     with pytest.raises(RuntimeError, match="pieces"):
         ops.page_fork(**a)
     assert all(torch.equal(a[k], v) for k, v in before.items())
+
+
+@pytest.mark.parametrize("sharers", [2, 3, 5])
+@pytest.mark.parametrize("free", [0, 1, 2, 4])
+def test_fork_serves_the_starved_with_as_many_pages(gpu, sharers, free):
+    import test_beams as cpu
+
+    a, want = cpu.starved_forks(sharers, free)
+    b = {k: [t.to(gpu) for t in v] if k == "pools" else v.to(gpu) for k, v in a.items()}
+    ops.page_fork(**b)
+    bref.page_fork(**a)
+    assert {k: b[k].tolist() for k in want} == want
+    assert torch.equal(a["pools"][0], b["pools"][0].cpu())
+
+
+def test_fork_of_many_that_share(gpu):
+    """Pages that slots of several parents go on in, some with a holder beside them, over tables of one launch and of two."""
+    for S, M, seed in ((60, 4, 1), (700, 9, 2), (2048, 3, 3)):
+        gen = torch.Generator().manual_seed(seed)
+        P = S + 50
+        shared = torch.randint(0, S // 3, (S,), generator=gen).to(torch.int32)  # the page that a slot goes on in
+        bt = torch.zeros(S, M, dtype=torch.int32)
+        bt[:, 0] = shared
+        refs = torch.bincount(shared.long(), minlength=P).to(torch.int32)
+        refs[: S // 3: 5] += 1
+        refs[S // 3: S // 3 + S // 4] = 1
+        parents = torch.where(torch.rand(S, generator=gen) < 0.8, torch.arange(S), torch.randint(-1, S, (S,), generator=gen))
+        state = [bt, torch.ones(S, dtype=torch.int32), torch.full((S,), 7, dtype=torch.int32)]
+        got = _fork(gpu, state, refs, parents.tolist(), [torch.randn(1, P, 8, generator=gen)])
+        assert int((got[5][:, 0] >= 0).sum()) > S // 4 and (S < 100 or int(got[6]) > 0)
