@@ -20,8 +20,12 @@ namespace {
 
 constexpr int kSelThreads = 512;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kGather = 1024;  // candidates that LDS holds; a chunk or group with more that reach the bound (many equal logits, the best
-                               // ones all in a few threads) is walked K times instead
+constexpr int kGather = 1024;  // candidates that LDS holds; a chunk or group with more that reach the bound (the best ones all in a few
+                               // threads) is walked K times instead
+// Where more buckets than this are as good as the K-th one, the bound lies among equals, as in a row that a finite value masks: it then
+// goes by their places too, or all of them would be gathered.  64x8 rows of 131072 bf16 with five tokens left: 38 us, 451 by a walk per
+// candidate; rows without equals 31 either way.
+constexpr int kTies = 16;
 
 // e^(x - m) for x <= m, by 2^y with y = (x - m) log2(e) in two parts
 DEV float exp_below(float x, float m) {
@@ -72,9 +76,9 @@ DEV V lane_value(V v, int lane) {  // a wave-uniform lane's value, without LDS
 }
 
 // The K-th largest of 64 buckets' maxima, the same for every thread; mine: this thread's maximum, bucket = lane.  Of the chunk's values
-// some 64 (H(64) - H(64 - K)) reach it: 1.1 K of them for K = 8, 1.4 K for 32, but 4.7 K for 64.
+// some 64 (H(64) - H(64 - K)) reach it: 1.1 K of them for K = 8, 1.4 K for 32, but 4.7 K for 64.  ties: buckets that equal it.
 template <typename V>
-DEV V bound_of_lanes(V mine, int K, V* all, int* rank) {
+DEV V bound_of_lanes(V mine, int K, V* all, int* rank, int& ties) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   all[threadIdx.x] = mine;
   if (wave == 0) rank[lane] = 0;
@@ -92,11 +96,13 @@ DEV V bound_of_lanes(V mine, int K, V* all, int* rank) {
   atomicAdd(&rank[lane], n);
   __syncthreads();
   const unsigned long long who = __ballot(rank[lane] == K - 1);
-  return lane_value(v, __ffsll(who) - 1);
+  const V bound = lane_value(v, __ffsll(who) - 1);
+  ties = __popcll(__ballot(v == bound));
+  return bound;
 }
 // The same with 128 buckets, where 64 would let too much through: 1.4 K for K = 64
 template <typename V>
-DEV V bound_of_many(V mine, int K, V* all, int* rank) {
+DEV V bound_of_many(V mine, int K, V* all, int* rank, int& ties) {
   constexpr int kBuckets = 128, kParts = kSelThreads / kBuckets, kEach = kBuckets / kParts;
   const int b = threadIdx.x % kBuckets, part = threadIdx.x / kBuckets;
   all[threadIdx.x] = mine;
@@ -115,7 +121,20 @@ DEV V bound_of_many(V mine, int K, V* all, int* rank) {
   __syncthreads();
   if (part == 0 && rank[b] == K - 1) all[kBuckets] = v;
   __syncthreads();
-  return all[kBuckets];
+  const V bound = all[kBuckets];
+  ties = __popcll(__ballot(all[threadIdx.x & 63] == bound)) + __popcll(__ballot(all[64 + (threadIdx.x & 63)] == bound));
+  return bound;
+}
+template <typename V>
+DEV V bound_of(V mine, int K, V* all, int* rank, int& ties) {
+  return K <= 32 ? bound_of_lanes(mine, K, all, rank, ties) : bound_of_many(mine, K, all, rank, ties);
+}
+// The place that the equals of such a bound count up to.  above, equal: whether this thread's maximum is above the bound or equals it;
+// place: of the first of this thread's values that equals it.  Called by every thread.
+DEV int last_place(bool above, bool equal, int place, int K, int* all, int* rank) {
+  int ties;
+  __syncthreads();  // everyone has read what the bound left in `all` and `rank`
+  return 0x7ffffffe - bound_of(above ? 0x7fffffff : (equal ? 0x7ffffffe - place : -1), K, all, rank, ties);
 }
 
 // Q: 16-byte pieces of a thread.  A row is whole pieces from its first element on, whatever address that has, and the few elements
@@ -190,7 +209,8 @@ __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectPar
   const float top = wave_max(ref);
   sum = wave_sum(sum * exp_below(ref, top));
   if (lane == 0) s_max[wave] = top, s_sum[wave] = sum;
-  const float bound = p.K <= 32 ? bound_of_lanes(m, p.K, bucket, rank) : bound_of_many(m, p.K, bucket, rank);
+  int ties;
+  const float bound = bound_of(m, p.K, bucket, rank, ties);
   if (threadIdx.x == 0) {
     float all = s_max[0], s = 0.f;
 #pragma unroll
@@ -200,23 +220,31 @@ __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectPar
     p.stat[(size_t)row * p.chunks + c] = make_float2(all, s);
   }
   // pieces that reach the bound are few: they are read again (from the caches), so that the registers need no index
-  auto gather = [&](float v, int token) {
-    if (v >= bound && v > -INFINITY && token != p.eos) {
+  int last = 0x7fffffff;  // piece that the bound's equals count up to; what is behind the whole pieces counts as the next one
+  if (ties > kTies && bound > -INFINITY) {
+    int first = pieces;
+#pragma unroll
+    for (int k = Q - 1; k >= 0; --k) first = most[k] == m ? place + k * kSelThreads : first;
+    last = last_place(m > bound, m == bound, first, p.K, reinterpret_cast<int*>(bucket), rank);
+  }
+  auto reaches = [&](float v, int piece) { return v >= bound && v > -INFINITY && (v > bound || piece <= last); };
+  auto gather = [&](float v, int piece, int token) {
+    if (reaches(v, piece) && token != p.eos) {
       const int at = atomicAdd(&count, 1);
       if (at < kGather) got[at] = logit_key(v, token);
     }
   };
   uint32_t hits = 0;
 #pragma unroll
-  for (int k = 0; k < Q; ++k) hits |= most[k] >= bound && most[k] > -INFINITY ? 1u << k : 0u;
-  if (extra_at >= 0) gather(extra, extra_at);
+  for (int k = 0; k < Q; ++k) hits |= reaches(most[k], place + k * kSelThreads) ? 1u << k : 0u;
+  if (extra_at >= 0) gather(extra, pieces, extra_at);
   while (hits) {
-    const int token = (place + (__ffs(hits) - 1) * kSelThreads) * N;
+    const int piece = place + (__ffs(hits) - 1) * kSelThreads, token = piece * N;
     hits &= hits - 1;
     Piece<T> h;
     h.load(x + token);
 #pragma unroll
-    for (int i = 0; i < N; ++i) gather(h.at(i), token + i);
+    for (int i = 0; i < N; ++i) gather(h.at(i), piece, token + i);
   }
   __syncthreads();
   const int n = count;
@@ -267,11 +295,12 @@ DEV int quotient(int n, float inv) { return (int)(((float)n + 0.5f) * inv); }
 
 __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParams p) {
   constexpr int kHeld = 8;             // candidates of a thread that its registers hold
+  constexpr int kNoted = kHeld * kSelThreads;  // lists that can be noted
   __shared__ double base[kBeamWidth];  // scores[row] - log(sum about `top`); NaN: the row offers nothing
   __shared__ float top[kBeamWidth];
   __shared__ double bucket[kSelThreads];
   __shared__ Pick got[kGather];
-  __shared__ int rank[128], count, open[kHeld * kSelThreads], nopen;
+  __shared__ int rank[128], count, open[kNoted], nopen;
   const int g = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) count = nopen = 0;
@@ -340,21 +369,28 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
   };
   double best = -INFINITY;
   each([&](const Pick& c, int, int) { best = c.s > best ? c.s : best; });
-  const double bound = p.K <= 32 ? bound_of_lanes(best, p.K, bucket, rank) : bound_of_many(best, p.K, bucket, rank);
+  int ties;
+  const double bound = bound_of(best, p.K, bucket, rank, ties);
+  int last = 0x7fffffff;  // id that the bound's equals count up to
+  if (ties > kTies && bound > -INFINITY) {
+    int first = 0x7ffffffe;
+    each([&](const Pick& c, int, int) { first = c.s == bound ? min(first, c.id) : first; });
+    last = last_place(best > bound, best == bound, first, p.K, reinterpret_cast<int*>(bucket), rank);
+  }
   auto gather = [&](const Pick& c) {
-    const bool in = c.s >= bound && c.s > -INFINITY;
-    if (in) {
+    if (c.s >= bound && c.s > -INFINITY && (c.s > bound || c.id <= last)) {
       const int at = atomicAdd(&count, 1);
       if (at < kGather) got[at] = c;
     }
-    return in;
   };
   if (best >= bound)
     each([&](const Pick& c, int list, int at) {
-      if (gather(c) && at == deep - 1 && deep < p.K) {
+      gather(c);
+      // by the score alone: of logits whose scores are equal the later one in a list may be the lower token
+      if (at == deep - 1 && deep < p.K && c.s >= bound && c.s > -INFINITY) {
         const int o = atomicAdd(&nopen, 1);
-        if (o < kHeld * kSelThreads) open[o] = list;
-        else count = kGather + 1;  // `got` has overflowed by then: place by place, below
+        if (o < kNoted) open[o] = list;
+        else atomicAdd(&count, kGather + 1);  // place by place, below
       }
     });
   __syncthreads();

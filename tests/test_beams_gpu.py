@@ -835,3 +835,70 @@ def test_fork_of_many_that_share(gpu):
         state = [bt, torch.ones(S, dtype=torch.int32), torch.full((S,), 7, dtype=torch.int32)]
         got = _fork(gpu, state, refs, parents.tolist(), [torch.randn(1, P, 8, generator=gen)])
         assert int((got[5][:, 0] >= 0).sum()) > S // 4 and (S < 100 or int(got[6]) > 0)
+
+
+def _masked(gen, rows, V, dtype, low, allowed):
+    """Rows of which `allowed` tokens are left (the first one among them), the others at a finite value."""
+    x = _logits(gen, rows, V, dtype)
+    keep = torch.zeros(rows, V, dtype=torch.bool)
+    for r in range(rows):
+        keep[r, torch.randperm(V, generator=gen)[: allowed]] = True
+    keep[:, 0] = allowed > 0
+    return torch.where(keep, x, torch.tensor(low, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low", ["lowest", -1e9, -16.0])
+@pytest.mark.parametrize("groups,width,V,K,allowed", [(2, 4, 33001, 16, 3), (1, 8, 5000, 64, 1), (3, 2, 40000, 5, 0), (1, 32, 7257, 58, 2),
+                                                     (4, 4, 2051, 33, 40)])
+def test_select_masked_by_a_finite_value(gpu, dtype, low, groups, width, V, K, allowed):
+    """Few tokens left in a row, the others equal: the rest of the places goes to the lowest of those."""
+    gen = torch.Generator().manual_seed(V + K)
+    logits = _masked(gen, groups * width, V, dtype, torch.finfo(dtype).min if low == "lowest" else low, allowed)
+    scores = _scores(gen, logits if allowed else torch.zeros_like(logits), groups, width, 9)
+    for eos in (-1, 2):
+        _same_choice(*_select(gpu, logits.to(gpu), scores, K, eos))
+
+
+def _microseconds(f):
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(5):
+            f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 200)
+    return sorted(times)[3]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("groups,width,V,K", [(64, 8, 131072, 16), (8, 32, 7257, 58), (16, 5, 50001, 10)])
+def test_select_of_masked_rows_takes_no_longer(gpu, dtype, groups, width, V, K):
+    """Equal logits do not cost a walk of the row per candidate."""
+    gen = torch.Generator(device=gpu).manual_seed(V)
+    x = (torch.randn(groups * width, V, device=gpu, generator=gen) * 2.5).to(dtype)
+    keep = torch.rand(groups * width, V, device=gpu, generator=gen) < 5 / V
+    scores = -torch.rand(groups, width, device=gpu, generator=gen)
+    o = (torch.zeros(groups, K, device=gpu), torch.zeros(groups, K, dtype=torch.int32, device=gpu),
+         torch.zeros(groups, K, dtype=torch.int32, device=gpu))
+    usual = _microseconds(lambda: ops.beam_select(x, scores, *o, 2))
+    for low in (torch.finfo(dtype).min, -1e9):
+        masked = torch.where(keep, x, torch.tensor(low, dtype=dtype, device=gpu))
+        assert _microseconds(lambda: ops.beam_select(masked, scores, *o, 2)) < 2 * usual + 5
+    equal = torch.full_like(x, 0.5)
+    assert _microseconds(lambda: ops.beam_select(equal, scores, *o, 2)) < 2 * usual + 5
+
+
+@pytest.mark.parametrize("dtype,piece", [(torch.float32, 4), (torch.bfloat16, 8)])
+@pytest.mark.parametrize("K,lanes", [(16, 9), (32, 20), (64, 40)])
+def test_select_best_in_few_lanes(gpu, dtype, piece, K, lanes):
+    """The best tokens all in the pieces that a few lanes read: more of them are above the bound than LDS holds."""
+    gen = torch.Generator().manual_seed(K)
+    V = 70000
+    logits = _logits(gen, 2, V, dtype) / 8
+    hot = torch.arange(V) // piece % (64 if K <= 32 else 128) < lanes
+    logits[:, hot] += 8
+    scores = _scores(gen, logits, 1, 2, 3)
+    _same_choice(*_select(gpu, logits.to(gpu), scores, K, 3))
