@@ -25,7 +25,8 @@ struct BeamSelectParams {
   int* out_rows;        // [groups, K] absolute rows, -1 where nothing is left
   int* out_tokens;      // [groups, K]
   float* end_scores;    // [rows] or null
-  float2* stat;         // [rows, chunks] maximum, sum of exponentials
+  double* sum;          // [rows, chunks] sum of exponentials about the maximum
+  float* most;          // [rows, chunks] maximum
   float2* cand;         // [rows, chunks, K] logit, token (bits); best first
   float* end_logit;     // [rows]
   int64_t ld;

@@ -9,7 +9,9 @@
 // merge  one workgroup per group: the chunks' sums joined into each row's log-sum, the same selection over the rows' candidates.
 //
 // Two candidates of different rows may be nearer to each other than 32 bits of a score of tens tell, so scores are compared in 64
-// bits, and the exponentials' argument carries the error of log2(e): a row's log-sum is off by some 1e-8, not 1e-6.
+// bits, the exponentials' argument carries the error of log2(e), and sums are joined in 64 bits from the wave on.  A row's log-sum is
+// off by 1e-8 to 3e-8 rms for 32768 tokens and more (by 1.2e-7 with every sum in 32 bits), 5e-8 for 1000; where all of a row's terms
+// are the same, by the rounding of their exponential, 1.2e-7.
 //
 // 64 groups of 8 rows of 131072 bf16 logits, 16 candidates: 35 to 36 us (3.8 TB/s), 29 without the selection, which the exponentials share the
 // vector units with; the merge 7.3.  One group of 4 rows of 32768 (fp32): 4.4 and 4.6 us, all latency.
@@ -144,7 +146,8 @@ DEV int last_place(bool above, bool equal, int place, int K, int* all, int* rank
 template <typename T, int Q>
 __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectParams p) {
   constexpr int N = Piece<T>::N;
-  __shared__ float s_max[kSelWaves], s_sum[kSelWaves];
+  __shared__ float s_max[kSelWaves];
+  __shared__ double s_sum[kSelWaves];
   __shared__ float bucket[kSelThreads];
   __shared__ int rank[128], count;
   __shared__ uint64_t got[kGather];
@@ -201,23 +204,33 @@ __global__ void __launch_bounds__(kSelThreads, 6) beam_rows_kernel(BeamSelectPar
     m = fmaxf(m, most[k]);
   }
   const float ref = fmaxf(fmaxf(m, end), -3.4028234663852886e38f);  // -inf alone sums to zero
-  float sum = exp_below(extra, ref) + exp_below(end, ref);
+  // a piece's sum, then the thread's, in 32 bits, everything behind it in 64: a likely token, beside which the others are rounded, is added
+  // to 7 + Q times, not to all of the thread's and then the wave's
+  float own = 0.f;
 #pragma unroll
-  for (int k = 0; k < Q; ++k)
+  for (int k = 0; k < Q; ++k) {
+    float part = exp_below(q[k].at(0), ref);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += exp_below(q[k].at(i), ref);
+    for (int i = 1; i < N; ++i) part += exp_below(q[k].at(i), ref);
+    own += part;
+  }
+  double sum = (double)own + ((double)exp_below(extra, ref) + exp_below(end, ref));
   const float top = wave_max(ref);
-  sum = wave_sum(sum * exp_below(ref, top));
+  sum *= exp_below(ref, top);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) s_max[wave] = top, s_sum[wave] = sum;
   int ties;
   const float bound = bound_of(m, p.K, bucket, rank, ties);
   if (threadIdx.x == 0) {
-    float all = s_max[0], s = 0.f;
+    float all = s_max[0];
+    double s = 0;
 #pragma unroll
     for (int w = 1; w < kSelWaves; ++w) all = fmaxf(all, s_max[w]);
 #pragma unroll
     for (int w = 0; w < kSelWaves; ++w) s += s_sum[w] * exp_below(s_max[w], all);
-    p.stat[(size_t)row * p.chunks + c] = make_float2(all, s);
+    p.most[(size_t)row * p.chunks + c] = all;
+    p.sum[(size_t)row * p.chunks + c] = s;
   }
   // pieces that reach the bound are few: they are read again (from the caches), so that the registers need no index
   int last = 0x7fffffff;  // piece that the bound's equals count up to; what is behind the whole pieces counts as the next one
@@ -325,14 +338,14 @@ __global__ void __launch_bounds__(kSelThreads) beam_merge_kernel(BeamSelectParam
   for (int i = 0; i < kHeld; ++i)
     if (i == 0 || i * kSelThreads < total) held[i] = load(min((int)threadIdx.x + i * kSelThreads, total - 1));
   for (int w = threadIdx.x >> 4; w < p.width; w += kSelThreads / 16) {  // 16 lanes per row
-    const float2* st = p.stat + (size_t)(g * p.width + w) * p.chunks;
+    const size_t at = (size_t)(g * p.width + w) * p.chunks;
     const int l = threadIdx.x & 15;
     float m = -INFINITY;
-    for (int c = l; c < p.chunks; c += 16) m = fmaxf(m, st[c].x);
+    for (int c = l; c < p.chunks; c += 16) m = fmaxf(m, p.most[at + c]);
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     double sum = 0;
-    for (int c = l; c < p.chunks; c += 16) sum += (double)st[c].y * exp((double)st[c].x - (double)m);
+    for (int c = l; c < p.chunks; c += 16) sum += p.sum[at + c] * exp((double)p.most[at + c] - (double)m);
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
     if (l == 0) {

@@ -84,12 +84,13 @@ void beam_select(const Tensor& logits, const Tensor& scores, Tensor& out_scores,
   p.f32 = logits.scalar_type() == at::kFloat ? 1 : 0;
   p.rows = (int)logits.size(0), p.width = (int)scores.size(1), p.V = (int)V, p.K = (int)K, p.eos = (int)eos_id;
   dsse_beam_plan_rows(&p);
-  // [statistics | candidates | end logits]
+  // [sums | candidates | maxima | end logits]
   const int64_t parts = (int64_t)p.rows * p.chunks;
-  Tensor work = at::empty({2 * parts * (1 + K) + p.rows}, scores.options());
-  p.stat = reinterpret_cast<float2*>(work.data_ptr<float>());
-  p.cand = p.stat + parts;
-  p.end_logit = work.data_ptr<float>() + 2 * parts * (1 + K);
+  Tensor work = at::empty({parts * (3 + 2 * K) + p.rows}, scores.options());
+  p.sum = reinterpret_cast<double*>(work.data_ptr<float>());
+  p.cand = reinterpret_cast<float2*>(p.sum + parts);
+  p.most = reinterpret_cast<float*>(p.cand + parts * K);
+  p.end_logit = p.most + parts;
   p.scores = scores.data_ptr<float>();
   p.out_scores = out_scores.data_ptr<float>();
   p.out_rows = out_rows.data_ptr<int>();

@@ -902,3 +902,52 @@ def test_select_best_in_few_lanes(gpu, dtype, piece, K, lanes):
     logits[:, hot] += 8
     scores = _scores(gen, logits, 1, 2, 3)
     _same_choice(*_select(gpu, logits.to(gpu), scores, K, 3))
+
+
+def _end_errors(gpu, x):
+    """By how much the scores of ending with token 1 are off, from base scores that bring them near zero, where they round by nothing."""
+    want = x[:, 1].double() - torch.logsumexp(x.double(), 1)
+    base = (-want).float().view(-1, 1)
+    end, o = torch.zeros_like(base), (torch.zeros(len(x), 1, device=gpu), torch.zeros(len(x), 1, dtype=torch.int32, device=gpu),
+                                      torch.zeros(len(x), 1, dtype=torch.int32, device=gpu))
+    ops.beam_select(x, base, *o, 1, end)
+    return end.view(-1).double() - (want + base.view(-1).double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("where", ["end", "candidate"])
+def test_select_log_sums(gpu, dtype, where):
+    """Half of a row's sum in one token, the other half in 131071.  A wave's sum is scaled by an exponential whose argument, up to 16,
+    rounds by 2^-21 at most, 2^-21 / sqrt(3) rms: 1.9e-7 of the value.  There are 32 waves at least, their errors independent, over
+    half of the sum: 1.9e-7 / sqrt(32) / 2 = 1.7e-8.  A candidate's exponential is added to in its thread, 15 times at most, by half a
+    step of a number from 1 to 2, 2^-24 / sqrt(3) rms: sqrt(15) 3.4e-8 / 2 = 6.7e-8 of the sum."""
+    rows, V = 64, 131072
+    x = (torch.randn(rows, V, device=gpu, generator=torch.Generator(device=gpu).manual_seed(1)) * 0.5).to(dtype)
+    x[:, 1] = -20.0
+    top = torch.logsumexp(x.double(), 1)
+    at = torch.randint(2, V, (rows,), device=gpu, generator=torch.Generator(device=gpu).manual_seed(2))
+    if where == "end":
+        at = torch.ones_like(at)
+    x[torch.arange(rows, device=gpu), at] = top.to(dtype)
+    rms = float(_end_errors(gpu, x).pow(2).mean().sqrt())
+    assert rms < (2.5e-8 if where == "end" else (1.7e-8 ** 2 + 6.7e-8 ** 2) ** 0.5), rms
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [40, 5000, 50001])
+def test_select_scores_a_step_apart(gpu, dtype, V):
+    """Rows of the same logits and base scores one 32-bit step apart, the best in the last row: in 32 bits the scores are the same."""
+    gen = torch.Generator().manual_seed(V)
+    row = torch.randn(V, generator=gen).clamp(-3, 3)
+    row[V // 2], row[V // 3] = 4.0, 3.5
+    W, K = 8, 16
+    logits = row.to(dtype).expand(W, V).contiguous()
+    base = torch.tensor([-0.7])
+    bases = [float(base)]
+    while len(bases) < W:
+        base = torch.nextafter(base, torch.zeros(1))
+        bases.append(float(base))
+    scores = torch.tensor([bases])
+    want, got = _select(gpu, logits.to(gpu), scores, K)
+    assert got[1].tolist() == [2 * list(range(W - 1, -1, -1))] and got[2].tolist() == [W * [V // 2] + W * [V // 3]]
+    assert torch.equal(want[1], got[1]) and torch.equal(want[2], got[2])
