@@ -35,7 +35,7 @@ constexpr int kDim = 128;
 constexpr int kHalf = kPg * kDim * 2;  // bytes of a page's keys, or of its values
 constexpr int kRing = 3;               // pages in LDS: three workgroups of a CU keep six pages on their way
 constexpr int kOwnWaves = 2;           // waves that split a slot's own pages
-constexpr float kLow = -1e30f;         // a finite start: fully masked columns stay finite and sum to zero
+constexpr float kLow = -3.4028234663852886e38f;  // a finite start, below any score: fully masked columns stay finite and sum to zero
 
 constexpr int waves_of(int T) { return T == 1 ? 4 : T; }
 

@@ -951,3 +951,21 @@ def test_select_scores_a_step_apart(gpu, dtype, V):
     want, got = _select(gpu, logits.to(gpu), scores, K)
     assert got[1].tolist() == [2 * list(range(W - 1, -1, -1))] and got[2].tolist() == [W * [V // 2] + W * [V // 3]]
     assert torch.equal(want[1], got[1]) and torch.equal(want[2], got[2])
+
+
+@pytest.mark.parametrize("width,hq,hkv", [(3, 4, 2), (6, 8, 2), (4, 16, 1), (10, 16, 1)])
+def test_attention_scores_far_below_zero(gpu, width, hq, hkv):
+    """Keys that all score -3.7e33: equal weights, over shared pages and a slot's own."""
+    gen = torch.Generator().manual_seed(width)
+    lens, common = [100 + 7 * s for s in range(width)], [2]
+    bt, pages = _tables(gen, lens, common, width)
+    _, v = _cache(gen, pages, hkv, "cpu")
+    k = torch.full((pages, hkv, 32, 128), -2.0 ** 54, dtype=torch.bfloat16)
+    q = torch.full((width, hq, 128), 2.0 ** 54, dtype=torch.bfloat16)
+    ctx, shared = torch.tensor(lens, dtype=torch.int32), torch.tensor(common, dtype=torch.int32)
+    out = torch.zeros_like(q).to(gpu)
+    ops.beam_attention(q.to(gpu), k.to(gpu), v.to(gpu), bt.to(gpu), ctx.to(gpu), shared.to(gpu), out, width)
+    for s, n in enumerate(lens):  # weights of one are exact: the result rounds, and its sum in 32 bits
+        V = gather_kv(k, v, bt[s], n)[1].double().repeat_interleave(hq // hkv, 1)
+        want = V.mean(0)
+        assert bool(((out[s].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + n * 2.0 ** -24 * V.abs().mean(0)).all())
