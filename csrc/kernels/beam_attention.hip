@@ -20,6 +20,10 @@
 // Measured, walks + join: 8x8 beams of 32 heads over 8 and some 8300 tokens 60 + 5 us (5.6 TB/s in the walks), 2x16 of 16 over 4 and
 // 31077 29 to 33 + 5, 16x4 of 612 15 + 4.  Each beam's pages read by themselves are 6 times the bytes in the first case, 15 in the second.
 //
+// Pages are read by non-temporal loads: a step reads every layer's pages and weights before it comes back to a layer's, so nothing of
+// them is left in the caches.  Over 32 layers in turn 16x4 beams of 612 tokens take 19.0 to 19.7 us so, 20.5 to 21.0 by default loads,
+// 8x8 of 8300 65 to 69 and 72 to 74, 2x16 of 31077 36 and 38; of one layer read again and again the first 20.8 and 19.3.
+//
 // Statistics and sums in fp32; scores in base 2 with the scale folded in; weights rounded to bf16 for the second product, as in
 // paged_attention.
 #include "api_beams.h"
@@ -114,10 +118,9 @@ DEV void blank_values(bf16x8 (&vf)[8], int left) {
 }
 
 // Keys of pages [pb, pe) up to `limit`, for 16 columns, pages in turn to NW waves
-template <int NW, bool ONCE>
+template <int NW>
 DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int limit, int row, Column& c) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
-  auto load = [](const bf16* at) { return ONCE ? ld_once<bf16x8>(at) : ld_global<bf16x8>(at); };
   bf16x8 qf[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) qf[k] = row >= 0 ? ld_bf16x8(p.q + (size_t)row * kDim + 32 * k + 8 * g) : zero_bf16x8();
@@ -131,11 +134,11 @@ DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int
     bf16x8 k0[4], k1[4], vf[8];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      k0[s] = load(kp + r * kDim + 32 * s + 8 * g);
-      k1[s] = load(kp + (16 + r) * kDim + 32 * s + 8 * g);
+      k0[s] = ld_once<bf16x8>(kp + r * kDim + 32 * s + 8 * g);
+      k1[s] = ld_once<bf16x8>(kp + (16 + r) * kDim + 32 * s + 8 * g);
     }
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) vf[dt] = load(vp + (16 * dt + r) * kPg + 8 * g);
+    for (int dt = 0; dt < 8; ++dt) vf[dt] = ld_once<bf16x8>(vp + (16 * dt + r) * kPg + 8 * g);
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -151,7 +154,7 @@ DEV void walk(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int
 }
 
 // The same for T column tiles, one per wave: whole pages [pb, pe) through LDS
-template <int T, bool ONCE>
+template <int T>
 DEV void walk_tiles(const BeamAttnParams& p, const int* bt, int h, int pb, int pe, int row, Column& c, char* smem) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // head dims of a k-step: 32 g + 8 s .. + 7 of both operands
@@ -182,7 +185,7 @@ DEV void walk_tiles(const BeamAttnParams& p, const int* bt, int h, int pb, int p
     char* to = smem + slot_in * 2 * kHalf + wave * IPW * 1024;
     slot_in = slot_in + 1 == kRing ? 0 : slot_in + 1;
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) lds_dma<ONCE ? kAuxNT : 0>(src, to + i * 1024, from[i]);
+    for (int i = 0; i < IPW; ++i) lds_dma<kAuxNT>(src, to + i * 1024, from[i]);
   };
   int kofs[4];
 #pragma unroll
@@ -274,7 +277,7 @@ DEV int2 part_of(int pages, int n, int z, int least) {
   return make_int2(pb, min(pages, pb + per));
 }
 
-template <int T, bool ONCE>
+template <int T>
 __global__ void __launch_bounds__(64 * waves_of(T), 2) beam_attention_kernel(BeamAttnParams p) {
   constexpr int NW = waves_of(T);
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -294,10 +297,10 @@ __global__ void __launch_bounds__(64 * waves_of(T), 2) beam_attention_kernel(Bea
     }
     const int* bt = p.block_tables + (size_t)live * p.max_blocks;
     if constexpr (T == 1) {
-      walk<NW, ONCE>(p, bt, h, part.x, part.y, part.y * kPg, row, c);
+      walk<NW>(p, bt, h, part.x, part.y, part.y * kPg, row, c);
       leave_joined<NW>(p, c, row, z, smem);
     } else {
-      walk_tiles<T, ONCE>(p, bt, h, part.x, part.y, row, c, smem);
+      walk_tiles<T>(p, bt, h, part.x, part.y, row, c, smem);
       leave(p, c, row, z);
     }
   } else {
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(64 * waves_of(T), 2) beam_attention_kernel(Bea
       if (lane < 16 && row >= 0) p.part_ml[(size_t)row * np + p.ns + z] = make_float2(kLow, 0.f);
       return;
     }
-    walk<kOwnWaves, ONCE>(p, p.block_tables + (size_t)s * p.max_blocks, h, skip + part.x, skip + part.y, n, row, c);
+    walk<kOwnWaves>(p, p.block_tables + (size_t)s * p.max_blocks, h, skip + part.x, skip + part.y, n, row, c);
     leave_joined<kOwnWaves>(p, c, row, p.ns + z, smem);
   }
 }
@@ -380,13 +383,7 @@ __global__ void __launch_bounds__(64) beam_shared_kernel(const int* tables, cons
   if (lane == 0) shared[g] = found;
 }
 
-// Pages of a layer that fill less than half of the 256 MB memory-side cache may still be there when they are read next; others only
-// wash it through, and non-temporal loads are the faster.  Measured, those against the default, three pools in turn: 64 MB each 26 / 24
-// us, 92 MB (16x4 beams of 612 tokens) 18.3 / 14.8, 95 MB 23.7 / 18.9, 134 MB (2x16 of 31077) 29.7 / 33.1, 300 MB 50 / 54, 371 MB (8x8
-// of 8300) 62 / 70.
-constexpr int64_t kStays = 112 << 20;
-
-template <int T, bool ONCE>
+template <int T>
 hipError_t launch_attention(dim3 grid, const BeamAttnParams& p, hipStream_t st) {
   constexpr int NW = waves_of(T), ring = T > 1 ? kRing * 2 * kHalf : 0, lds = ring > join_bytes(NW) ? ring : join_bytes(NW);
   if (lds > 64 * 1024) {  // once per device
@@ -395,12 +392,12 @@ hipError_t launch_attention(dim3 grid, const BeamAttnParams& p, hipStream_t st) 
     hipError_t e = hipGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (e == hipSuccess && !(set.load(std::memory_order_relaxed) & bit)) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&beam_attention_kernel<T, ONCE>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&beam_attention_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (e == hipSuccess) set.fetch_or(bit, std::memory_order_relaxed);
     }
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((beam_attention_kernel<T, ONCE>), grid, dim3(64 * NW), lds, st, p);
+  hipLaunchKernelGGL((beam_attention_kernel<T>), grid, dim3(64 * NW), lds, st, p);
   return hipGetLastError();
 }
 
@@ -432,12 +429,11 @@ extern "C" hipError_t dsse_beam_attention(const dsse::BeamAttnParams* p, hipStre
   const int groups = p->slots / p->width;
   const int per = waves_of(p->tiles) / kOwnWaves;  // own walks of a workgroup
   const dim3 grid((groups * p->col_blocks * p->ns + (p->slots * p->no + per - 1) / per) * p->hkv);
-  const bool once = (int64_t)p->num_blocks * p->hkv * 2 * kHalf > kStays;
   hipError_t e = hipErrorInvalidValue;
-  if (p->tiles == 1) e = once ? launch_attention<1, true>(grid, *p, st) : launch_attention<1, false>(grid, *p, st);
-  else if (p->tiles == 2) e = once ? launch_attention<2, true>(grid, *p, st) : launch_attention<2, false>(grid, *p, st);
-  else if (p->tiles == 4) e = once ? launch_attention<4, true>(grid, *p, st) : launch_attention<4, false>(grid, *p, st);
-  else if (p->tiles == 8) e = once ? launch_attention<8, true>(grid, *p, st) : launch_attention<8, false>(grid, *p, st);
+  if (p->tiles == 1) e = launch_attention<1>(grid, *p, st);
+  else if (p->tiles == 2) e = launch_attention<2>(grid, *p, st);
+  else if (p->tiles == 4) e = launch_attention<4>(grid, *p, st);
+  else if (p->tiles == 8) e = launch_attention<8>(grid, *p, st);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(beam_join_kernel, dim3((p->slots * p->hq + 3) / 4), dim3(256), 0, st, *p);
   return hipGetLastError();

@@ -969,3 +969,31 @@ def test_attention_scores_far_below_zero(gpu, width, hq, hkv):
         V = gather_kv(k, v, bt[s], n)[1].double().repeat_interleave(hq // hkv, 1)
         want = V.mean(0)
         assert bool(((out[s].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + n * 2.0 ** -24 * V.abs().mean(0)).all())
+
+
+@pytest.mark.parametrize("width,hq", [(4, 4), (8, 12), (16, 16), (20, 24), (32, 16)])
+def test_attention_in_a_large_pool(gpu, width, hq):
+    """A cache allocated ahead, its live pages anywhere in it, and tables as wide as the longest sequence: the same numbers."""
+    gen = torch.Generator().manual_seed(width + hq)
+    lens, common = [0 if s % 7 == 3 else 400 + 3 * s for s in range(2 * width)], [11, 0]
+    bt, small = _tables(gen, lens, common, width)
+    k, v = (x.to(gpu) for x in _cache(gen, small, 4, "cpu"))
+    pages = 2500  # 164 MB
+    bk, bv = torch.full((pages, 4, 32, 128), math.nan, dtype=torch.bfloat16, device=gpu), torch.full((pages, 4, 128, 32), math.nan, dtype=torch.bfloat16, device=gpu)
+    at = torch.randperm(pages, generator=gen)[:small]
+    bk[at], bv[at] = k, v
+    wide = torch.full((2 * width, 1025), -1, dtype=torch.int32)
+    wide[:, : bt.shape[1]] = at[bt.long()].to(torch.int32)
+    q = torch.randn(2 * width, hq, 128, generator=gen).to(torch.bfloat16).to(gpu)
+    ctx, shared = torch.tensor(lens, dtype=torch.int32, device=gpu), torch.tensor(common, dtype=torch.int32, device=gpu)
+    out = torch.full_like(q, 3.0)
+    ops.beam_attention(q, bk, bv, wide.to(gpu), ctx, shared, out, width)
+    for s, n in enumerate(lens):
+        got = out[s].cpu().double()
+        if n == 0:
+            assert bool((got == 3.0).all())
+            continue
+        K, V = (x.double().repeat_interleave(hq // 4, 1) for x in gather_kv(k.cpu(), v.cpu(), bt[s], n))
+        p = torch.softmax((q[s].cpu().double()[None] * K).sum(-1) / math.sqrt(128), 0)[..., None]
+        want, size = (p * V).sum(0), (p * V.abs()).sum(0)
+        assert bool(((got - want).abs() <= (2.0 ** -8 + 1e-4) * size + 2.0 ** -8 * want.abs()).all()), s
