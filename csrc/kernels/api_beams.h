@@ -10,6 +10,7 @@ namespace dsse {
 constexpr int kBeamWidth = 32;  // beams of a group
 constexpr int kBeamKeep = 64;   // candidates of a group
 constexpr int kForkSlots = 2048;
+constexpr int kSharedSlots = (1 << 26) - 1;  // slots whose common pages are counted: a grid's threads, 64 a group, stay in 32 bits
 constexpr int kReorderLists = 96;  // tensors of one launch (24 bytes each of a kernel's arguments)
 constexpr int kCopyPools = 64;     // (32 bytes each)
 constexpr int kCopyPage = 1 << 30;     // bytes of a page in a layer: offsets past its end, of whole work items, stay in 32 bits

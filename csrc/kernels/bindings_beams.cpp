@@ -149,6 +149,7 @@ void beam_shared(const Tensor& block_tables, const Tensor& ctx_len, int64_t widt
   typed(ctx_len, block_tables, at::kInt, "ctx_len");
   typed(shared, block_tables, at::kInt, "shared");
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(1) >= 1 && block_tables.size(1) < (1 << 26), "block_tables must be [slots, max_blocks]");
+  TORCH_CHECK(block_tables.size(0) <= dsse::kSharedSlots, "at most ", dsse::kSharedSlots, " slots");
   const int groups = beams(block_tables.size(0), width);
   TORCH_CHECK(ctx_len.numel() == block_tables.size(0) && shared.numel() == groups, "ctx_len must be [slots], shared [groups]");
   if (groups == 0) return;

@@ -39,7 +39,7 @@ def beam_select(logits, scores, out_scores, out_rows, out_tokens, eos_id: int = 
 
 def beam_shared(block_tables, ctx_len, width: int, shared):
     """shared [groups] = how many leading whole pages (of all ctx_len tokens) the tables of a group's live slots have in common;
-    0 without a live slot (ctx_len 0 = idle).  Once per step, for all layers."""
+    0 without a live slot (ctx_len 0 = idle).  Once per step, for all layers.  At most 2^26 - 1 slots."""
     if _hip(block_tables):
         torch.ops.dsse.beam_shared(block_tables, ctx_len, width, shared)
     else:

@@ -9,7 +9,7 @@ import torch
 from .reference import PAGE, gather_kv
 
 BEAM_WIDTH, BEAM_KEEP, FORK_SLOTS, BEAM_ROWS = 32, 64, 2048, 1 << 22
-COPY_PIECE, COPY_PIECES = 1 << 14, (1 << 31) - 1
+COPY_PIECE, COPY_PIECES, SHARED_SLOTS = 1 << 14, (1 << 31) - 1, (1 << 26) - 1
 
 
 def _need(ok: bool, text: str) -> None:
@@ -74,6 +74,7 @@ def beam_shared(block_tables, ctx_len, width, shared):
     for t, n in ((block_tables, "block_tables"), (ctx_len, "ctx_len"), (shared, "shared")):
         _typed(t, torch.int32, n)
     _need(block_tables.dim() == 2 and block_tables.shape[1] >= 1, "block_tables must be [slots, max_blocks]")
+    _need(block_tables.shape[0] <= SHARED_SLOTS, f"at most {SHARED_SLOTS} slots")
     G = _beams(block_tables.shape[0], width)
     _need(ctx_len.numel() == block_tables.shape[0] and shared.numel() == G, "ctx_len must be [slots], shared [groups]")
     for g in range(G):

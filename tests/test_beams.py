@@ -361,3 +361,9 @@ def test_fork_serves_the_starved_with_as_many_pages(sharers, free):
     assert {k: a[k].tolist() for k in want} == want
     for old, new in want["copies"]:
         assert old < 0 or torch.equal(a["pools"][0][:, new], a["pools"][0][:, old])
+
+
+def test_shared_of_too_many_slots():
+    e = torch.empty(1 << 26, 1, dtype=i32)  # nothing reads it
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.beam_shared(e, e.view(-1), 1, e.view(-1))

@@ -997,3 +997,9 @@ def test_attention_in_a_large_pool(gpu, width, hq):
         p = torch.softmax((q[s].cpu().double()[None] * K).sum(-1) / math.sqrt(128), 0)[..., None]
         want, size = (p * V).sum(0), (p * V.abs()).sum(0)
         assert bool(((got - want).abs() <= (2.0 ** -8 + 1e-4) * size + 2.0 ** -8 * want.abs()).all()), s
+
+
+def test_shared_of_too_many_slots(gpu):
+    e = torch.empty(1 << 26, 1, dtype=torch.int32, device=gpu)  # nothing reads it
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.beam_shared(e, e.view(-1), 1, e.view(-1))
