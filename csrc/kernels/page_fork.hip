@@ -144,9 +144,10 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
     }
     mask |= 1 << i;
   }
+  int wanted, rank = block_scan(__popc(mask) | ask << 16, scan, wanted);  // of up to 2048 slots; above them, whether any asks
   // Slots of several parents go on in one page where an earlier call found no free one.  That is rare, so all slots are looked through
   // then: if they alone hold it, the last of them keeps it.
-  if (__syncthreads_or(ask)) {
+  if (wanted >> 16) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if (shared_by[i] < 0) continue;
@@ -155,10 +156,8 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(PageForkParams
         if (goes_to[t] == page[i]) ++n, end = t;
       if (n == shared_by[i] && end == s0 + i) mask &= ~(1 << i);
     }
+    rank = block_scan(__popc(mask), scan, wanted);
   }
-  const int need = __popc(mask);
-  int wanted;
-  int rank = block_scan(need, scan, wanted);
   // the lowest free pages, as many as are wanted
   int found = 0;
   for (int base = 0; base < p.pages && found < wanted; base += kForkThreads * 4) {
