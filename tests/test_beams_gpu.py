@@ -1003,3 +1003,24 @@ def test_shared_of_too_many_slots(gpu):
     e = torch.empty(1 << 26, 1, dtype=torch.int32, device=gpu)  # nothing reads it
     with pytest.raises(RuntimeError, match="at most"):
         ops.beam_shared(e, e.view(-1), 1, e.view(-1))
+
+
+@pytest.mark.parametrize("width,hq", [(4, 4), (6, 12), (9, 16), (20, 16)])
+def test_attention_more_shared_pages_than_whole_ones(gpu, width, hq):
+    """Counts past the whole pages of every slot are those, negative ones none, with 1 to 8 column tiles."""
+    gen = torch.Generator().manual_seed(width)
+    k, v = _cache(gen, 12, 2, gpu)
+    bt = torch.randperm(12, generator=gen).to(torch.int32).expand(width, 12).contiguous().to(gpu)
+    q = torch.randn(width, hq, 128, generator=gen).to(torch.bfloat16).to(gpu)
+    ctx = torch.tensor([290 + s for s in range(width)], dtype=torch.int32, device=gpu)
+    outs = []
+    for n in (9, 10, 10 ** 6, 2 ** 31 - 1, 0, -3, -2 ** 31):
+        outs.append(torch.zeros_like(q))
+        ops.beam_attention(q, k, v, bt, ctx, torch.tensor([n], dtype=torch.int32, device=gpu), outs[-1], width)
+    assert all(torch.equal(outs[0], o) for o in outs[1:4]) and all(torch.equal(outs[4], o) for o in outs[5:])
+    for s in range(width):
+        K, V = (x.double().repeat_interleave(hq // 2, 1) for x in gather_kv(k.cpu(), v.cpu(), bt[s].cpu(), 290 + s))
+        p = torch.softmax((q[s].cpu().double()[None] * K).sum(-1) / math.sqrt(128), 0)[..., None]
+        want, size = (p * V).sum(0), (p * V.abs()).sum(0)
+        for o in (outs[0], outs[4]):
+            assert bool(((o[s].cpu().double() - want).abs() <= (2.0 ** -8 + 1e-4) * size + 2.0 ** -8 * want.abs()).all()), s
