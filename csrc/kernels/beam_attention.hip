@@ -14,11 +14,12 @@
 // T = 1 (up to 16 columns): four waves take the pages in turn, straight to registers, and join their sums in LDS; a slot's own pages
 // go to two waves in the same way, several slots to a workgroup.
 // T = 2, 4, 8: a wave per column tile; the pages pass through LDS once for all waves, filled by LDS-DMA kRing - 1 pages ahead.  A
-// page costs 16 KB from memory and T tiles' products, so what bounds it is memory.  A ring of 5 pages lets one workgroup on a CU
-// where one of 3 lets three: 2x16 beams of 31077 tokens 36 -> 28.6 us.
+// page costs 16 KB from memory and T tiles' products, so what bounds it is memory.  A ring of 5 pages lets fewer workgroups on a CU
+// than one of 3, which lets three of T = 2 or 4: 2x16 beams of 31077 tokens 36 -> 28.6 us.  T = 8 has one by its registers, 142 in each
+// of eight waves, and two pages on their way: 19x16 beams of 32 heads over 4 and some 985 tokens 56 + 7 us (2.9 TB/s in the walks).
 //
 // Measured, walks + join: 8x8 beams of 32 heads over 8 and some 8300 tokens 60 + 5 us (5.6 TB/s in the walks), 2x16 of 16 over 4 and
-// 31077 29 to 33 + 5, 16x4 of 612 15 + 4.  Each beam's pages read by themselves are 6 times the bytes in the first case, 15 in the second.
+// 31077 29 to 33 + 5, 16x4 of 612 17 + 4.5.  Each beam's pages read by themselves are 6 times the bytes in the first case, 15 in the second.
 //
 // Pages are read by non-temporal loads: a step reads every layer's pages and weights before it comes back to a layer's, so nothing of
 // them is left in the caches.  Over 32 layers in turn 16x4 beams of 612 tokens take 19.0 to 19.7 us so, 20.5 to 21.0 by default loads,
@@ -37,7 +38,7 @@ namespace {
 constexpr int kPg = 32;
 constexpr int kDim = 128;
 constexpr int kHalf = kPg * kDim * 2;  // bytes of a page's keys, or of its values
-constexpr int kRing = 3;               // pages in LDS: three workgroups of a CU keep six pages on their way
+constexpr int kRing = 3;               // pages in LDS: three workgroups of a CU (T = 8: one) keep two pages each on their way
 constexpr int kOwnWaves = 2;           // waves that split a slot's own pages
 constexpr float kLow = -3.4028234663852886e38f;  // a finite start, below any score: fully masked columns stay finite and sum to zero
 
@@ -406,7 +407,8 @@ hipError_t launch_attention(dim3 grid, const BeamAttnParams& p, hipStream_t st) 
 
 // Column tiles of a workgroup and cuts of the walks, from what the host knows: the lengths are on the device, so the tables' width
 // stands for them.  Shared walks: a workgroup per CU where it holds four tiles or more (4x16 beams of 16 heads and 16077 tokens
-// 28.9 us with 16 parts, 35 with 32), two where it holds fewer.  Own walks: eight waves per CU.
+// 28.9 us with 16 parts, 35 with 32), two where it holds fewer.  Own walks: four waves per CU, two a walk.  Tables of 1025 columns in
+// place of the sequences' own cost 2 to 5 % of short walks (1x4 beams of 700 tokens 10.1 -> 10.4 us) and nothing of long ones.
 extern "C" void dsse_beam_plan(dsse::BeamAttnParams* p) {
   using namespace dsse;
   const int cols = p->width * p->group, groups = p->slots / p->width;

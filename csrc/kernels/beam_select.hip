@@ -13,8 +13,9 @@
 // off by 1e-8 to 3e-8 rms for 32768 tokens and more (by 1.2e-7 with every sum in 32 bits), 5e-8 for 1000; where all of a row's terms
 // are the same, by the rounding of their exponential, 1.2e-7.
 //
-// 64 groups of 8 rows of 131072 bf16 logits, 16 candidates: 35 to 36 us (3.8 TB/s), 29 without the selection, which the exponentials share the
-// vector units with; the merge 7.3.  One group of 4 rows of 32768 (fp32): 4.4 and 4.6 us, all latency.
+// 64 groups of 8 rows of 131072 bf16 logits, 16 candidates: 35 us (3.8 TB/s; 31 of logits that the caches still hold in part), 29 without
+// the selection, which the exponentials share the vector units with; the merge 7.4 to 7.9.  One group of 4 rows of 32768 (fp32): 4.4 and
+// 4.6 to 5.0 us, all latency.
 #include "api_beams.h"
 
 namespace dsse {
